@@ -34,6 +34,7 @@ extern "C" {
 #define SAD_SRC_IDS 0  /* int64 token ids [B,T]                  (reference: self.embedding(src)) */
 #define SAD_SRC_F32 1  /* fp32 soft tokens [B,T,V]               (reference: src @ embedding.weight) */
 #define SAD_SRC_BF16 2 /* bf16 soft tokens [B,T,V] */
+#define SAD_SRC_F16 3  /* fp16; only the gated scan and the 8-bit checkpoints take it */
 
 typedef struct sad_dims {
     int32_t B; /* sentences in this call */
@@ -344,6 +345,66 @@ int sad_soft_finalize(int32_t B, int32_t T, int32_t V, int32_t steps, int32_t ov
                       int32_t eos_id, void* S, int32_t s_kind, int64_t s_stride_t, int64_t s_stride_b, int64_t* ids,
                       float* val, const int32_t* lens_steps, const uint8_t* alive, int32_t* lens_out, uint8_t* mask,
                       void* stream);
+
+/* ---- gated linear recurrence -----------------------------------------------------------------------------
+ * A recurrence beside the LSTM / GRU whose state is one number per channel, so that it can be cut along time: no
+ * limit on T, no hand-off inside the launch (no counterpart in the reference).  z = [x | f | o] holds the
+ * pre-activations of D channels (gated == 0: [x | f]), e.g. one linear layer's output:
+ *     s_t = sigmoid(-f_t),  h_t = h_{t-1} + s_t (x_t - h_{t-1}),  y_t = sigmoid(o_t) h_t      for t < lengths[b]
+ * in time order, or from t = lengths[b] - 1 down to 0 (reverse).  y is 0 and the state unchanged at t >= lengths[b];
+ * such rows of z and dy are not used, and dz is 0 there.  State and sums are fp32.
+ * The last axis of z, y, dy, dz has unit stride; rows are addressed through element strides; h0, h_last, dh_last, dh0 are
+ * dense [B,D]. */
+typedef struct sad_scan_args {
+    int32_t B, T, D;          /* D >= 2 channels */
+    int32_t kind;             /* SAD_SRC_F32 / _BF16 / _F16: z, y, dy, dz */
+    int32_t gated;            /* 1: z has an output gate */
+    int32_t reverse;
+    const void* z;            /* [B,T,3D] or [B,T,2D]; the backward pass reads it only where codes is NULL */
+    int64_t z_stride_b, z_stride_t;
+    const int32_t* lengths;   /* [B] or NULL (every sentence has T tokens); clamped to 0..T */
+    const float* h0;          /* [B,D] or NULL (0) */
+    void* y;                  /* out [B,T,D] */
+    int64_t y_stride_b, y_stride_t;
+    float* h_last;            /* out [B,D]: the state after the last token */
+    float* kept;              /* sad_gated_scan_kept_bytes: the state entering every 16 steps; NULL in a forward without
+                                 gradients */
+    void* codes;              /* sad_gated_scan_codes_bytes, 16-byte aligned, or NULL.  Given, the forward pass keeps z
+                                 in 8 bits there (the checkpoints' number format, each of x, f, o a matrix of its own) and
+                                 the backward pass differentiates the recurrence at those values */
+    /* backward */
+    const void* dy;           /* [B,T,D] or NULL (0) */
+    int64_t dy_stride_b, dy_stride_t;
+    const float* dh_last;     /* [B,D] or NULL (0) */
+    void* dz;                 /* out, the shape of z */
+    int64_t dz_stride_b, dz_stride_t;
+    float* dh0;               /* out [B,D] or NULL */
+} sad_scan_args;
+size_t sad_gated_scan_workspace_bytes(int32_t B, int32_t T, int32_t D);
+size_t sad_gated_scan_kept_bytes(int32_t B, int32_t T, int32_t D);
+size_t sad_gated_scan_codes_bytes(int32_t B, int32_t T, int32_t D, int32_t gated);
+int sad_gated_scan_fwd(const sad_scan_args* a, void* workspace, void* stream);
+int sad_gated_scan_bwd(const sad_scan_args* a, void* workspace, void* stream);
+/* One token of it: z [B,3D] / [B,2D] and the states h [B,D] -> y [B,D], h_out [B,D] (fp32; h_out may be h).  `alive` as in
+ * sad_gumbel_args: a sentence that has ended keeps its state and gives y = 0. */
+int sad_gated_scan_step(int32_t B, int32_t D, int32_t kind, int32_t gated, const void* z, int64_t z_stride_b, const float* h,
+                        int64_t h_stride_b, const uint8_t* alive, void* y, int64_t y_stride_b, float* h_out, int64_t h_out_stride_b,
+                        void* stream);
+
+/* ---- 8-bit activation checkpoints ---------------------------------------------------------------------------
+ * A matrix [rows, C] as int8 codes with one exponent e per row and 32 channels: the smallest e with
+ * max|x| <= 127 * 2^e over the finite entries (kept within [-126, 122], fp16 [-24, 10]); an entry stands for
+ * rint(x / 2^e) * 2^e, a non-finite one for NaN.  `saved` holds sad_checkpoint8_bytes, 16-byte aligned.
+ * Rows are those of a [n0,n1,C] tensor with unit channel stride and the given element strides, in that order. */
+size_t sad_checkpoint8_bytes(int64_t rows, int64_t C);
+int sad_checkpoint8_save(int64_t n0, int64_t n1, int64_t C, int32_t kind, const void* x, int64_t stride0, int64_t stride1,
+                         void* saved, void* stream);
+int sad_checkpoint8_restore(int64_t rows, int64_t C, int32_t kind, const void* saved, void* out, void* stream);
+/* dw [N,K] = dy^T x^ (and db [N] = column sums of dy, or NULL) with dy [n0,n1,N] and x^ the values of a checkpoint of
+ * n0 * n1 rows of K channels; fp32 sums, the same result at every call. */
+size_t sad_weight_grad8_workspace_bytes(int64_t rows, int64_t N, int64_t K);
+int sad_weight_grad8(int64_t n0, int64_t n1, int64_t N, int64_t K, int32_t kind, const void* dy, int64_t stride0, int64_t stride1,
+                     const void* saved, float* dw, float* db, void* workspace, void* stream);
 
 /* Test / diagnosis settings (process-wide; no counterpart in the reference).  Do not change them
  * between a sad_forward and its sad_backward.

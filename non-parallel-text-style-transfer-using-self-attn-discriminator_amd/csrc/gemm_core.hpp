@@ -160,6 +160,15 @@ __device__ __forceinline__ u32x4 load_row(const bf16raw* row, bool ok, const bf1
     return u32x4{0u, 0u, 0u, 0u};
 }
 
+// 8 k-values (rows r .. r+3 and r+16 .. r+19 of a 32-row slab) of one column of a row-major LDS tile; see wgrad.hpp.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ bf16x8 tr_frag(const unsigned char* p, int pitch) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * pitch));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 struct Ident {
     __device__ __forceinline__ u32x4 operator()(u32x4 v) const { return v; }
 };

@@ -1,6 +1,7 @@
 // libsad host side: C-ABI entry points (include/sad.h), layouts, argument checks, launches.
 // gfx950 only.  Nothing here allocates, frees or synchronises.
 #include "../../include/sad.h"
+#include "host.hpp"
 #include "kernels.hpp"
 #include "wgrad.hpp"
 #include "wgrad2.hpp"
@@ -33,6 +34,22 @@ int fail(int code, const char* fmt, ...) {
     va_end(ap);
     return code;
 }
+
+}  // namespace
+
+namespace sad {
+
+int set_error(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+}  // namespace sad
+
+namespace {
 
 #define SAD_CHECK_LAUNCH(name)                                                          \
     do {                                                                                \

@@ -1,0 +1,304 @@
+// C-ABI entry points of the gated linear recurrence and of the 8-bit activation checkpoints (include/sad.h).
+// gfx950 only.  Nothing here allocates, frees or synchronises, and nothing needs zeroed workspaces.
+#include "../../include/sad.h"
+#include "host.hpp"
+#include "scan.hpp"
+#include "ckpt8.hpp"
+#include "wgrad8.hpp"
+
+using namespace sad;
+
+namespace {
+
+#define SAD_LAUNCHED(name)                                                                   \
+    do {                                                                                     \
+        hipError_t e__ = hipGetLastError();                                                  \
+        if (e__ != hipSuccess) return set_error(-2, "%s: %s", name, hipGetErrorString(e__)); \
+    } while (0)
+#define SAD_NEED(ptr, name)                                             \
+    do {                                                                \
+        if ((ptr) == nullptr) return set_error(-1, "%s is NULL", name); \
+    } while (0)
+
+constexpr int MAX_GRID = 0x7fffffff;
+
+bool known_kind(int kind) { return kind == SAD_SRC_F32 || kind == SAD_SRC_BF16 || kind == SAD_SRC_F16; }
+
+// ---- scan ---------------------------------------------------------------------------------------------------------
+// Time chunks of a sentence: one where the waves of all sentences and channel groups fill the card by themselves.
+int scan_chunks(int B, int T, int D) {
+    const long long waves = (long long)B * ceil_div(D, SC_CH);
+    const int nblk = ceil_div(T, SC_STEPS);
+    if (waves >= 1024) return 1;
+    long long n = (2048 + waves - 1) / waves;
+    if (n > 64) n = 64;
+    if (n > nblk) n = nblk;
+    const int cblk = ceil_div(nblk, (int)n);
+    return ceil_div(nblk, cblk);
+}
+
+int check_scan_dims(int B, int T, int D, int kind) {
+    if (B < 1 || T < 1 || D < 2) return set_error(-1, "gated scan needs B >= 1, T >= 1, D >= 2 (B=%d T=%d D=%d)", B, T, D);
+    if (D > (1 << 24) || T > (1 << 28)) return set_error(-1, "gated scan: D=%d or T=%d beyond the supported maximum", D, T);
+    if ((long long)B * ceil_div(D, SC_CH) * 64 > MAX_GRID) return set_error(-1, "gated scan: B=%d x D=%d beyond the supported maximum", B, D);
+    if (!known_kind(kind)) return set_error(-1, "kind must be SAD_SRC_F32, SAD_SRC_BF16 or SAD_SRC_F16, got %d", kind);
+    return 0;
+}
+
+ScanP scan_params(const sad_scan_args* a, void* workspace) {
+    ScanP p{};
+    p.B = a->B; p.T = a->T; p.D = a->D;
+    p.nblk = ceil_div(a->T, SC_STEPS);
+    p.ncg = ceil_div(a->D, SC_CH);
+    p.reverse = a->reverse != 0;
+    p.nchunk = scan_chunks(a->B, a->T, a->D);
+    p.cblk = ceil_div(p.nblk, p.nchunk);
+    p.z = a->z; p.z_sb = a->z_stride_b; p.z_st = a->z_stride_t;
+    p.lengths = a->lengths;
+    p.h0 = a->h0;
+    p.y = a->y; p.y_sb = a->y_stride_b; p.y_st = a->y_stride_t;
+    p.h_last = a->h_last;
+    p.kept = a->kept;
+    p.codes = (unsigned char*)a->codes;
+    if (a->codes != nullptr)
+        p.exps = p.codes + (size_t)a->B * p.nblk * (a->gated ? 3 : 2) * a->D * SC_STEPS;
+    p.dy = a->dy; p.dy_sb = a->dy_stride_b; p.dy_st = a->dy_stride_t;
+    p.dh_last = a->dh_last;
+    p.dz = a->dz; p.dz_sb = a->dz_stride_b; p.dz_st = a->dz_stride_t;
+    p.dh0 = a->dh0;
+    p.sums = (float*)workspace;
+    return p;
+}
+
+int scan_grid(const ScanP& p) { return (int)(((long long)p.B * p.ncg * p.nchunk + 3) / 4); }
+
+template <int KIND>
+int launch_scan_fwd(const sad_scan_args* a, const ScanP& p, hipStream_t st) {
+    const dim3 grid(scan_grid(p)), block(256);
+    if (p.nchunk > 1) {
+        hipLaunchKernelGGL((k_scan_sum<KIND>), grid, block, 0, st, p);
+        SAD_LAUNCHED("k_scan_sum");
+    }
+    const int save = p.codes != nullptr ? 2 : (p.kept != nullptr ? 1 : 0);
+#define SCAN_FWD(G, S) hipLaunchKernelGGL((k_scan_fwd<KIND, G, S>), grid, block, 0, st, p)
+    if (a->gated) {
+        if (save == 0) SCAN_FWD(true, 0);
+        else if (save == 1) SCAN_FWD(true, 1);
+        else SCAN_FWD(true, 2);
+    } else {
+        if (save == 0) SCAN_FWD(false, 0);
+        else if (save == 1) SCAN_FWD(false, 1);
+        else SCAN_FWD(false, 2);
+    }
+#undef SCAN_FWD
+    SAD_LAUNCHED("k_scan_fwd");
+    return 0;
+}
+
+template <int KIND, bool GATED, bool CODES>
+int launch_scan_bwd(const ScanP& p, hipStream_t st) {
+    const dim3 grid(scan_grid(p)), block(256);
+    if (p.nchunk > 1) {
+        hipLaunchKernelGGL((k_scan_bsum<KIND, GATED, CODES>), grid, block, 0, st, p);
+        SAD_LAUNCHED("k_scan_bsum");
+    }
+    hipLaunchKernelGGL((k_scan_bwd<KIND, GATED, CODES>), grid, block, 0, st, p);
+    SAD_LAUNCHED("k_scan_bwd");
+    return 0;
+}
+
+template <int KIND>
+int launch_scan_bwd(const sad_scan_args* a, const ScanP& p, hipStream_t st) {
+    if (a->gated) return p.codes != nullptr ? launch_scan_bwd<KIND, true, true>(p, st) : launch_scan_bwd<KIND, true, false>(p, st);
+    return p.codes != nullptr ? launch_scan_bwd<KIND, false, true>(p, st) : launch_scan_bwd<KIND, false, false>(p, st);
+}
+
+#define BY_KIND(kind, call)                                   \
+    do {                                                      \
+        if ((kind) == SAD_SRC_F32) { constexpr int KIND = SAD_SRC_F32; call; }        \
+        else if ((kind) == SAD_SRC_BF16) { constexpr int KIND = SAD_SRC_BF16; call; } \
+        else { constexpr int KIND = SAD_SRC_F16; call; }                              \
+    } while (0)
+
+// ---- checkpoints ----------------------------------------------------------------------------------------------------
+int check_matrix(int64_t rows, int64_t C, int kind) {
+    if (rows < 1 || C < 1) return set_error(-1, "rows and channels must be positive (rows=%lld C=%lld)", (long long)rows, (long long)C);
+    if (rows > MAX_GRID || C > (1 << 24)) return set_error(-1, "rows=%lld or C=%lld beyond the supported maximum", (long long)rows, (long long)C);
+    if (!known_kind(kind)) return set_error(-1, "kind must be SAD_SRC_F32, SAD_SRC_BF16 or SAD_SRC_F16, got %d", kind);
+    return 0;
+}
+
+// ---- weight gradient --------------------------------------------------------------------------------------------------
+struct Split { int tn, tk, splits, rows; };
+// Row splits: enough workgroups for two rounds of the card's 256 CUs, no split shorter than 512 rows.
+Split wgrad8_split(int64_t M, int64_t N, int64_t K) {
+    Split s;
+    s.tn = (int)((N + W8_BN - 1) / W8_BN);
+    s.tk = (int)((K + W8_BK - 1) / W8_BK);
+    const int64_t tiles = (int64_t)s.tn * s.tk;
+    int64_t n = (512 + tiles - 1) / tiles, most = (M + 511) / 512;
+    if (n > most) n = most;
+    if (n < 1) n = 1;
+    int64_t rows = (M + n - 1) / n;
+    rows = (rows + W8_BM - 1) / W8_BM * W8_BM;
+    s.rows = (int)rows;
+    s.splits = (int)((M + rows - 1) / rows);
+    return s;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sad_gated_scan_workspace_bytes(int32_t B, int32_t T, int32_t D) {
+    if (check_scan_dims(B, T, D, SAD_SRC_F32)) return 0;
+    const int n = scan_chunks(B, T, D);
+    return n > 1 ? (size_t)B * n * 2 * D * sizeof(float) : 16;
+}
+
+size_t sad_gated_scan_kept_bytes(int32_t B, int32_t T, int32_t D) {
+    if (check_scan_dims(B, T, D, SAD_SRC_F32)) return 0;
+    return (size_t)B * ceil_div(T, SC_STEPS) * D * sizeof(float);
+}
+
+size_t sad_gated_scan_codes_bytes(int32_t B, int32_t T, int32_t D, int32_t gated) {
+    if (check_scan_dims(B, T, D, SAD_SRC_F32)) return 0;
+    return (size_t)B * ceil_div(T, SC_STEPS) * (gated ? 3 : 2) * ((size_t)D + ceil_div(D, C8_BLOCK)) * SC_STEPS;
+}
+
+int sad_gated_scan_fwd(const sad_scan_args* a, void* workspace, void* stream) {
+    SAD_NEED(a, "args");
+    if (check_scan_dims(a->B, a->T, a->D, a->kind)) return -1;
+    SAD_NEED(a->z, "z");
+    SAD_NEED(a->y, "y");
+    SAD_NEED(a->h_last, "h_last");
+    SAD_NEED(workspace, "workspace");
+    if (a->codes != nullptr && a->kept == nullptr) return set_error(-1, "codes need kept");
+    if ((size_t)a->codes % 16) return set_error(-1, "codes must be 16-byte aligned");
+    const ScanP p = scan_params(a, workspace);
+    BY_KIND(a->kind, return launch_scan_fwd<KIND>(a, p, (hipStream_t)stream));
+}
+
+int sad_gated_scan_bwd(const sad_scan_args* a, void* workspace, void* stream) {
+    SAD_NEED(a, "args");
+    if (check_scan_dims(a->B, a->T, a->D, a->kind)) return -1;
+    if (a->z == nullptr && a->codes == nullptr) return set_error(-1, "need z or codes");
+    SAD_NEED(a->kept, "kept");
+    SAD_NEED(a->dz, "dz");
+    SAD_NEED(workspace, "workspace");
+    if ((size_t)a->codes % 16) return set_error(-1, "codes must be 16-byte aligned");
+    const ScanP p = scan_params(a, workspace);
+    BY_KIND(a->kind, return launch_scan_bwd<KIND>(a, p, (hipStream_t)stream));
+}
+
+int sad_gated_scan_step(int32_t B, int32_t D, int32_t kind, int32_t gated, const void* z, int64_t z_stride_b, const float* h,
+                        int64_t h_stride_b, const uint8_t* alive, void* y, int64_t y_stride_b, float* h_out, int64_t h_out_stride_b,
+                        void* stream) {
+    if (B < 1 || D < 1) return set_error(-1, "B and D must be positive (B=%d D=%d)", B, D);
+    const int per = ceil_div(D, 256);
+    if ((int64_t)B * per > MAX_GRID) return set_error(-1, "B=%d x D=%d beyond the supported maximum", B, D);
+    if (!known_kind(kind)) return set_error(-1, "kind must be SAD_SRC_F32, SAD_SRC_BF16 or SAD_SRC_F16, got %d", kind);
+    SAD_NEED(z, "z");
+    SAD_NEED(h, "h");
+    SAD_NEED(y, "y");
+    SAD_NEED(h_out, "h_out");
+    const dim3 grid((unsigned)B * per);
+#define SCAN_STEP(G)                                                                                                          \
+    hipLaunchKernelGGL((k_scan_step<KIND, G>), grid, dim3(256), 0, (hipStream_t)stream, D, per, z, (long long)z_stride_b, h,   \
+                       (long long)h_stride_b, alive, y, (long long)y_stride_b, h_out, (long long)h_out_stride_b)
+    if (gated) BY_KIND(kind, SCAN_STEP(true));
+    else BY_KIND(kind, SCAN_STEP(false));
+#undef SCAN_STEP
+    SAD_LAUNCHED("k_scan_step");
+    return 0;
+}
+
+size_t sad_checkpoint8_bytes(int64_t rows, int64_t C) {
+    if (check_matrix(rows, C, SAD_SRC_F32)) return 0;
+    const size_t nb = (size_t)((C + C8_BLOCK - 1) / C8_BLOCK);
+    return (size_t)rows * nb * (C8_BLOCK + 1);
+}
+
+int sad_checkpoint8_save(int64_t n0, int64_t n1, int64_t C, int32_t kind, const void* x, int64_t stride0, int64_t stride1,
+                         void* saved, void* stream) {
+    if (n0 < 1 || n1 < 1) return set_error(-1, "rows must be positive (%lld x %lld)", (long long)n0, (long long)n1);
+    if (n0 > MAX_GRID || n1 > MAX_GRID) return set_error(-1, "rows beyond the supported maximum");
+    const int64_t rows = n0 * n1;
+    if (check_matrix(rows, C, kind)) return -1;
+    SAD_NEED(x, "x");
+    SAD_NEED(saved, "saved");
+    if ((size_t)saved % 16) return set_error(-1, "saved must be 16-byte aligned");
+    const int nb = (int)((C + C8_BLOCK - 1) / C8_BLOCK), per = 2 * nb, rpb = per < 256 ? 256 / per : 1;
+    unsigned char* codes = (unsigned char*)saved;
+    unsigned char* exps = codes + (size_t)rows * nb * C8_BLOCK;
+    const Rows2 xr{stride0, stride1, (unsigned)n1};
+    BY_KIND(kind, hipLaunchKernelGGL((k_ckpt8_save<KIND>), dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream,
+                                     (int)rows, (int)C, per, rpb, x, xr, codes, exps));
+    SAD_LAUNCHED("k_ckpt8_save");
+    return 0;
+}
+
+int sad_checkpoint8_restore(int64_t rows, int64_t C, int32_t kind, const void* saved, void* out, void* stream) {
+    if (check_matrix(rows, C, kind)) return -1;
+    SAD_NEED(saved, "saved");
+    SAD_NEED(out, "out");
+    if ((size_t)saved % 16) return set_error(-1, "saved must be 16-byte aligned");
+    const int nb = (int)((C + C8_BLOCK - 1) / C8_BLOCK), per = 2 * nb, rpb = per < 256 ? 256 / per : 1;
+    const unsigned char* codes = (const unsigned char*)saved;
+    const unsigned char* exps = codes + (size_t)rows * nb * C8_BLOCK;
+    BY_KIND(kind, hipLaunchKernelGGL((k_ckpt8_restore<KIND>), dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0,
+                                     (hipStream_t)stream, (int)rows, (int)C, per, rpb, codes, exps, out));
+    SAD_LAUNCHED("k_ckpt8_restore");
+    return 0;
+}
+
+size_t sad_weight_grad8_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
+    if (check_matrix(rows, K, SAD_SRC_F32) || check_matrix(rows, N, SAD_SRC_F32)) return 0;
+    const Split s = wgrad8_split(rows, N, K);
+    return s.splits > 1 ? (size_t)s.splits * (N * K + N) * sizeof(float) : 16;
+}
+
+int sad_weight_grad8(int64_t n0, int64_t n1, int64_t N, int64_t K, int32_t kind, const void* dy, int64_t stride0, int64_t stride1,
+                     const void* saved, float* dw, float* db, void* workspace, void* stream) {
+    if (n0 < 1 || n1 < 1) return set_error(-1, "rows must be positive (%lld x %lld)", (long long)n0, (long long)n1);
+    if (n0 > MAX_GRID || n1 > MAX_GRID) return set_error(-1, "rows beyond the supported maximum");
+    const int64_t M = n0 * n1;
+    if (check_matrix(M, K, kind) || check_matrix(M, N, kind)) return -1;
+    SAD_NEED(dy, "dy");
+    SAD_NEED(saved, "saved");
+    SAD_NEED(dw, "dw");
+    SAD_NEED(workspace, "workspace");
+    if ((size_t)saved % 16) return set_error(-1, "saved must be 16-byte aligned");
+    const Split s = wgrad8_split(M, N, K);
+    const int64_t groups = (int64_t)s.tn * s.tk * s.splits;
+    if (groups > MAX_GRID) return set_error(-1, "N=%lld x K=%lld beyond the supported maximum", (long long)N, (long long)K);
+    Wgrad8P p{};
+    p.M = (int)M; p.N = (int)N; p.K = (int)K;
+    p.Kp = (int)((K + C8_BLOCK - 1) / C8_BLOCK * C8_BLOCK);
+    p.dy = dy;
+    p.yr = Rows2{stride0, stride1, (unsigned)n1};
+    p.y_flat = n0 == 1 || stride0 == n1 * stride1;
+    p.codes = (const unsigned char*)saved;
+    p.exps = p.codes + (size_t)M * p.Kp;
+    p.tn = s.tn; p.tk = s.tk; p.splits = s.splits; p.rows = s.rows;
+    float* part_b = (float*)workspace + (size_t)s.splits * N * K;
+    p.out = s.splits > 1 ? (float*)workspace : dw;
+    p.out_b = db == nullptr ? nullptr : (s.splits > 1 ? part_b : db);
+    hipStream_t st = (hipStream_t)stream;
+    BY_KIND(kind, hipLaunchKernelGGL((k_wgrad8<KIND>), dim3((unsigned)groups), dim3(256), W8<KIND>::LDS, st, p));
+    SAD_LAUNCHED("k_wgrad8");
+    if (s.splits > 1) {
+        const long long n = (long long)N * K;
+        long long g = (n + 255) / 256;
+        hipLaunchKernelGGL(k_wgrad8_join, dim3((unsigned)(g < 8192 ? g : 8192)), dim3(256), 0, st, n, s.splits, (const float*)workspace, dw);
+        SAD_LAUNCHED("k_wgrad8_join");
+        if (db != nullptr) {
+            hipLaunchKernelGGL(k_wgrad8_join, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, (long long)N, s.splits,
+                               (const float*)part_b, db);
+            SAD_LAUNCHED("k_wgrad8_join");
+        }
+    }
+    return 0;
+}
+
+}  // extern "C"

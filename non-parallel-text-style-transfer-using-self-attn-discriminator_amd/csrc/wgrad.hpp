@@ -24,8 +24,6 @@
 
 namespace sad {
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
 template <int BN1_, int BN2_, int W1_, int W2_>
 struct WCfg {
     static constexpr int BN1 = BN1_, BN2 = BN2_, W1 = W1_, W2 = W2_, BK = 64;
@@ -39,14 +37,6 @@ struct WCfg {
     static_assert(BN1_ % (W1_ * 16) == 0 && BN2_ % (W2_ * 16) == 0, "tile/wave mismatch");
     static_assert((BK * CPR1) % NT == 0 && (BK * CPR2) % NT == 0, "staging must divide evenly");
 };
-
-// 8 k-values (rows r .. r+3 and r+16 .. r+19 of the slab) of one column; see file header.
-__device__ __forceinline__ bf16x8 tr_frag(const unsigned char* p, int pitch) {
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * pitch));
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
 
 // The reduction runs over a COMPACTED list of contributing token rows (k_row_lists): 45 % of the
 // rows of a ragged batch are padding and are never touched, and every 64-row tile is full, so the

@@ -656,3 +656,356 @@ def soft_embedding(soft_tokens, weight):
     :1221 content alignment).  bf16 MFMA inputs, fp32 accumulation; the result is rounded to bf16
     once (the kernels' activation format) and returned in the dtype of ``soft_tokens``."""
     return _SoftEmbedding.apply(soft_tokens, weight)
+
+
+# ------------------------------------------------------------------------------------------------
+# Gated linear recurrence (include/sad.h, sad_gated_scan_*): a recurrence beside the LSTM / GRU of the
+# discriminator whose state is one number per channel.  It has no product with the state, so its steps need no
+# exchange between workgroups and a long sentence is cut along time.
+# ------------------------------------------------------------------------------------------------
+_KINDS = {torch.float32: _lib.SRC_F32, torch.bfloat16: _lib.SRC_BF16, torch.float16: _lib.SRC_F16}
+
+
+def _kind(t, what):
+    kind = _KINDS.get(t.dtype)
+    if kind is None:
+        raise RuntimeError("%s must be float32, bfloat16 or float16, got %s" % (what, t.dtype))
+    return kind
+
+
+def _need_device(t, what):
+    if not t.is_cuda:
+        raise RuntimeError("%s must be on the HIP device (got a CPU tensor); there is no CPU path" % what)
+
+
+def _bytes(nbytes, what, dev):
+    """Uninitialised device memory of a size the library names (0 = it refused)."""
+    if nbytes == 0:
+        raise RuntimeError("libsad %s failed: %s" % (what, _lib.last_error()))
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+
+def _like_rows(t, last):
+    """New tensor [.., .., last] of t's type with the order of t's first two axes in memory."""
+    if t.stride(0) < t.stride(1) and t.shape[0] > 1 and t.shape[1] > 1:
+        return torch.empty((t.shape[1], t.shape[0], last), dtype=t.dtype, device=t.device).transpose(0, 1)
+    return torch.empty((t.shape[0], t.shape[1], last), dtype=t.dtype, device=t.device)
+
+
+def _scan_parts(width, gated_output):
+    parts = 3 if gated_output else 2
+    if width % parts or width < 2 * parts:
+        raise RuntimeError("z must hold %s of D >= 2 channels each along its last axis, got %d columns"
+                           % ("[x | f | o]" if gated_output else "[x | f]", width))
+    return width // parts
+
+
+def _scan_lengths(lengths, B, T, dev):
+    """int32 [B] on the device.  Unlike the LSTM's lengths they may be 0 and come in any order; values on the host are
+    checked, values on the device are clamped to 0..T by the kernels."""
+    if not torch.is_tensor(lengths):
+        lengths = torch.as_tensor(lengths)
+    if lengths.dim() != 1 or lengths.numel() != B or lengths.dtype.is_floating_point or lengths.dtype in (torch.bool, torch.complex64):
+        raise RuntimeError("lengths must be %d integers, got %s of shape %s" % (B, lengths.dtype, tuple(lengths.shape)))
+    if not lengths.is_cuda:
+        ln = lengths.detach().numpy()
+        if B > 0 and (int(ln.min()) < 0 or int(ln.max()) > T):
+            raise RuntimeError("lengths must lie in 0..%d, got %d..%d" % (T, int(ln.min()), int(ln.max())))
+    elif lengths.device != dev:
+        raise RuntimeError("lengths are on %s, z is on %s" % (lengths.device, dev))
+    elif lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, T)               # before it is narrowed
+    return lengths.to(device=dev, dtype=torch.int32, non_blocking=True).contiguous()
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, h0, lengths, reverse, gated, int8, track):
+        B, T = z.shape[:2]
+        D = z.shape[2] // (3 if gated else 2)
+        dev = z.device
+        lib = _lib.load()
+        y = _like_rows(z, D)
+        h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
+        kept = codes = None
+        ws = _bytes(lib.sad_gated_scan_workspace_bytes(B, T, D), "sad_gated_scan_workspace_bytes", dev)
+        if track:
+            kept = _bytes(lib.sad_gated_scan_kept_bytes(B, T, D), "sad_gated_scan_kept_bytes", dev)
+            if int8:
+                codes = _bytes(lib.sad_gated_scan_codes_bytes(B, T, D, gated), "sad_gated_scan_codes_bytes", dev)
+        a = _lib.SadScanArgs()
+        a.B, a.T, a.D, a.kind, a.gated, a.reverse = B, T, D, _KINDS[z.dtype], int(gated), int(reverse)
+        a.z, a.z_stride_b, a.z_stride_t = z.data_ptr(), z.stride(0), z.stride(1)
+        a.lengths = lengths.data_ptr() if lengths is not None else None
+        a.h0 = h0.data_ptr() if h0 is not None else None
+        a.y, a.y_stride_b, a.y_stride_t = y.data_ptr(), y.stride(0), y.stride(1)
+        a.h_last = h_last.data_ptr()
+        a.kept = kept.data_ptr() if kept is not None else None
+        a.codes = codes.data_ptr() if codes is not None else None
+        with _on(dev):
+            _lib.check(lib.sad_gated_scan_fwd(ctypes.byref(a), _ptr(ws), _stream_ptr()), "sad_gated_scan_fwd")
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(None if int8 else z, lengths, kept, codes)
+        ctx.scan = (B, T, D, z.dtype, tuple(z.shape), tuple(z.stride()), dev, reverse, gated)
+        return y, h_last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh_last):
+        z, lengths, kept, codes = ctx.saved_tensors
+        B, T, D, dtype, zshape, zstride, dev, reverse, gated = ctx.scan
+        if dy is None and dh_last is None:
+            return (None,) * 7
+        if dy is not None and dy.stride(2) != 1:
+            dy = dy.contiguous()
+        if dh_last is not None:
+            dh_last = dh_last.contiguous()
+        if _is_dense(zshape, zstride):
+            dz = torch.empty_strided(zshape, zstride, dtype=dtype, device=dev)
+        else:
+            dz = torch.empty(zshape, dtype=dtype, device=dev)
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
+        lib = _lib.load()
+        ws = _bytes(lib.sad_gated_scan_workspace_bytes(B, T, D), "sad_gated_scan_workspace_bytes", dev)
+        a = _lib.SadScanArgs()
+        a.B, a.T, a.D, a.kind, a.gated, a.reverse = B, T, D, _KINDS[dtype], int(gated), int(reverse)
+        if z is not None:
+            a.z, a.z_stride_b, a.z_stride_t = z.data_ptr(), z.stride(0), z.stride(1)
+        a.lengths = lengths.data_ptr() if lengths is not None else None
+        a.kept = kept.data_ptr()
+        a.codes = codes.data_ptr() if codes is not None else None
+        if dy is not None:
+            a.dy, a.dy_stride_b, a.dy_stride_t = dy.data_ptr(), dy.stride(0), dy.stride(1)
+        a.dh_last = dh_last.data_ptr() if dh_last is not None else None
+        a.dz, a.dz_stride_b, a.dz_stride_t = dz.data_ptr(), dz.stride(0), dz.stride(1)
+        a.dh0 = dh0.data_ptr() if dh0 is not None else None
+        with _on(dev):
+            _lib.check(lib.sad_gated_scan_bwd(ctypes.byref(a), _ptr(ws), _stream_ptr()), "sad_gated_scan_bwd")
+        return (dz if ctx.needs_input_grad[0] else None, dh0) + (None,) * 5
+
+
+def gated_scan(z, h0=None, lengths=None, reverse=False, gated_output=True, save="input"):
+    """Gated linear recurrence over a batch of sentences: ``(y [B,T,D], h_last [B,D])``.
+
+        s_t = sigmoid(-f_t)        h_t = h_{t-1} + s_t (x_t - h_{t-1})        y_t = sigmoid(o_t) h_t
+
+    ``z`` holds the pre-activations ``[x | f | o]`` as ``[B,T,3D]`` (``gated_output=False``: ``[x | f]``, ``[B,T,2D]``,
+    y = h), float32 / bfloat16 / float16, any batch and time strides with unit channel stride (the output of one linear
+    layer; time-major storage as a transposed view); y and the gradient come back in the same type and axis order.
+    ``h0`` [B,D] float32 is the state in front of the first token (default 0), ``h_last`` float32 the one after the last: a
+    long text can be read in pieces.  ``lengths`` [B] (host or device, 0..T, any order): y is 0 at t >= length, the state
+    stays, and such rows of z may hold anything.  ``reverse`` runs from the last token to the first.
+
+    Differentiable in z and h0.  ``save="input"`` keeps z for the backward pass; ``save="int8"`` keeps its 8-bit codes
+    instead (``checkpoint8``'s format, x, f and o separately) and gives the gradient at the restored values; both keep the
+    state entering every 16 tokens in float32, and a step between them is recomputed from there."""
+    _kind(z, "z")
+    if z.dim() != 3:
+        raise RuntimeError("z must be [B,T,3D] or [B,T,2D], got %s" % (tuple(z.shape),))
+    if save not in ("input", "int8"):
+        raise RuntimeError("save must be 'input' or 'int8', got %r" % (save,))
+    D = _scan_parts(z.shape[2], gated_output)
+    B, T = z.shape[:2]
+    if h0 is not None:
+        if h0.dtype != torch.float32 or tuple(h0.shape) != (B, D) or h0.device != z.device:
+            raise RuntimeError("h0 must be float32 [%d,%d] on %s, got %s %s on %s"
+                               % (B, D, z.device, h0.dtype, tuple(h0.shape), h0.device))
+    if lengths is not None:
+        lengths = _scan_lengths(lengths, B, T, z.device)
+    _need_device(z, "z")
+    if B == 0 or T == 0:
+        y = z[..., :D] * 1
+        return y, (h0.clone() if h0 is not None else torch.zeros((B, D), dtype=torch.float32, device=z.device))
+    if z.stride(2) != 1:
+        z = z.contiguous()
+    track = torch.is_grad_enabled() and (z.requires_grad or (h0 is not None and h0.requires_grad))
+    return _GatedScan.apply(z, h0.contiguous() if h0 is not None else None, lengths, bool(reverse), bool(gated_output),
+                            save == "int8", track)
+
+
+def _overlaps(a, b):
+    """Do the address ranges of two tensors meet?"""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
+    """One token of ``gated_scan`` for a decode loop: ``(y [B,D], h_out [B,D])``.
+
+    ``z`` [B,3D] / [B,2D] are the token's pre-activations, ``h`` [B,D] float32 the states.  The new states go to ``h_out``
+    (a new tensor if None; ``h`` itself updates in place).  ``alive`` [B] bool: a sentence that has ended keeps its state
+    and gives y = 0.  No gradient (train with ``gated_scan``)."""
+    kind = _kind(z, "z")
+    if z.dim() != 2:
+        raise RuntimeError("z must be [B,3D] or [B,2D], got %s" % (tuple(z.shape),))
+    D = _scan_parts(z.shape[1], gated_output)
+    B, dev = z.shape[0], z.device
+    if torch.is_grad_enabled() and (z.requires_grad or h.requires_grad):
+        raise RuntimeError("gated_scan_step has no gradient: call it under torch.no_grad(), or train with gated_scan")
+    for t, name in ((h, "h"), (h_out, "h_out")):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, D) or t.device != dev or t.stride(1) != 1):
+            raise RuntimeError("%s must be float32 [%d,%d] with unit channel stride on %s" % (name, B, D, dev))
+    if alive is not None and (alive.dtype not in (torch.bool, torch.uint8) or tuple(alive.shape) != (B,) or alive.device != dev):
+        raise RuntimeError("alive must be a bool [%d] tensor on %s" % (B, dev))
+    if h_out is None:
+        h_out = torch.empty((B, D), dtype=torch.float32, device=dev)
+    elif B and (B > 1 and h_out.stride(0) < D):
+        raise RuntimeError("rows of h_out overlap")
+    elif B and (h_out.data_ptr(), h_out.stride()) != (h.data_ptr(), h.stride()) and _overlaps(h_out, h):
+        raise RuntimeError("h_out must be h itself or must not overlap it")
+    if B and _overlaps(h_out, z):
+        raise RuntimeError("h_out must not overlap z")
+    _need_device(z, "z")
+    y = torch.empty((B, D), dtype=z.dtype, device=dev)
+    if B == 0:
+        return y, h_out
+    if z.stride(1) != 1:
+        z = z.contiguous()
+    if alive is not None:
+        alive = alive.contiguous()
+    with _on(dev):
+        _lib.check(_lib.load().sad_gated_scan_step(B, D, kind, int(gated_output), _ptr(z), z.stride(0), _ptr(h), h.stride(0), _ptr(alive),
+                                                   _ptr(y), y.stride(0), _ptr(h_out), h_out.stride(0), _stream_ptr()),
+                   "sad_gated_scan_step")
+    return y, h_out
+
+
+# ------------------------------------------------------------------------------------------------
+# 8-bit activation checkpoints (include/sad.h, sad_checkpoint8_*, sad_weight_grad8)
+# ------------------------------------------------------------------------------------------------
+def _rows2(t):
+    """(t, n0, n1, stride0, stride1): the rows of t [..., C] in their order, without a copy where two strides say it."""
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        t = t.contiguous()
+    if t.dim() > 3:
+        t = t.flatten(0, -2)
+    if t.dim() == 2:
+        return t, 1, t.shape[0], 0, t.stride(0)
+    return t, t.shape[0], t.shape[1], t.stride(0), t.stride(1)
+
+
+class Checkpoint8:
+    """A tensor [..., C] kept in 8 bits (``checkpoint8``): ``saved`` (uint8: codes, then exponents), ``shape``, ``dtype``."""
+
+    def __init__(self, saved, shape, dtype):
+        self.saved, self.shape, self.dtype = saved, torch.Size(shape), dtype
+
+    def restore(self):
+        """The values the codes stand for, as a new contiguous tensor of the original type."""
+        out = torch.empty(self.shape, dtype=self.dtype, device=self.saved.device)
+        if out.numel():
+            C = self.shape[-1]
+            with _on(out.device):
+                _lib.check(_lib.load().sad_checkpoint8_restore(out.numel() // C, C, _KINDS[self.dtype], _ptr(self.saved), _ptr(out),
+                                                               _stream_ptr()), "sad_checkpoint8_restore")
+        return out
+
+
+def checkpoint8(x):
+    """Keep ``x`` [..., C] (float32 / bfloat16 / float16) in 8 bits: int8 codes with one power-of-two step per row and 32
+    channels, the smallest whose 127 steps reach the largest finite entry.  An entry comes back within half a step (at most
+    1/127 of that largest entry; 1/63 where the type's own largest values leave no room above); infinities and NaN come
+    back as NaN and leave their neighbours alone.  Returns a ``Checkpoint8``; no gradient flows through it."""
+    kind = _kind(x, "x")
+    if x.dim() == 0:
+        raise RuntimeError("x must have a channel axis")
+    _need_device(x, "x")
+    shape, dev = x.shape, x.device
+    x = x.detach()
+    if x.numel() == 0:
+        return Checkpoint8(torch.empty(0, dtype=torch.uint8, device=dev), shape, x.dtype)
+    x, n0, n1, s0, s1 = _rows2(x)
+    C = shape[-1]
+    lib = _lib.load()
+    saved = _bytes(lib.sad_checkpoint8_bytes(n0 * n1, C), "sad_checkpoint8_bytes", dev)
+    with _on(dev):
+        _lib.check(lib.sad_checkpoint8_save(n0, n1, C, kind, _ptr(x), s0, s1, _ptr(saved), _stream_ptr()), "sad_checkpoint8_save")
+    return Checkpoint8(saved, shape, x.dtype)
+
+
+def weight_grad8(dy, ckpt, bias=False):
+    """Weight gradient ``dW [N,K] = dy^T x^`` (float32) of a linear layer from the checkpoint of its input ``x`` [..., K];
+    ``dy`` [..., N] has x's leading shape and type.  ``bias=True`` adds ``db [N] = sum dy``: ``(dW, db)``.  Sums are
+    float32 in a fixed order: the same call gives the same bits."""
+    kind = _kind(dy, "dy")
+    if dy.dtype != ckpt.dtype or dy.dim() != len(ckpt.shape) or dy.shape[:-1] != ckpt.shape[:-1]:
+        raise RuntimeError("dy %s %s does not belong to a checkpoint of %s %s"
+                           % (dy.dtype, tuple(dy.shape), ckpt.dtype, tuple(ckpt.shape)))
+    dev = dy.device
+    if ckpt.saved.device != dev:
+        raise RuntimeError("dy is on %s, the checkpoint on %s" % (dev, ckpt.saved.device))
+    _need_device(dy, "dy")
+    N, K = dy.shape[-1], ckpt.shape[-1]
+    dy = dy.detach()
+    if dy.numel() == 0 or K == 0:
+        dw = torch.zeros((N, K), dtype=torch.float32, device=dev)
+        if not bias:
+            return dw
+        return dw, (torch.zeros(N, dtype=torch.float32, device=dev) if dy.numel() == 0 else dy.float().flatten(0, -2).sum(0))
+    dy, n0, n1, s0, s1 = _rows2(dy)
+    lib = _lib.load()
+    dw = torch.empty((N, K), dtype=torch.float32, device=dev)
+    db = torch.empty(N, dtype=torch.float32, device=dev) if bias else None
+    ws = _bytes(lib.sad_weight_grad8_workspace_bytes(n0 * n1, N, K), "sad_weight_grad8_workspace_bytes", dev)
+    with _on(dev):
+        _lib.check(lib.sad_weight_grad8(n0, n1, N, K, kind, _ptr(dy), s0, s1, _ptr(ckpt.saved), _ptr(dw), _ptr(db), _ptr(ws),
+                                        _stream_ptr()), "sad_weight_grad8")
+    return (dw, db) if bias else dw
+
+
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        w = weight.to(x.dtype)
+        b = bias.to(x.dtype) if bias is not None else None
+        # a time-major activation seen as [B,T,K]: the product runs on its rows as they lie in memory
+        swap = x.dim() == 3 and not x.is_contiguous() and x.transpose(0, 1).is_contiguous()
+        xr = (x.transpose(0, 1) if swap else x).reshape(-1, x.shape[-1])
+        y = torch.nn.functional.linear(xr, w, b)
+        ctx.saved8 = None
+        saved = None
+        if ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2]):
+            ck = checkpoint8(x)
+            saved, ctx.saved8 = ck.saved, (ck.shape, ck.dtype)
+        ctx.save_for_backward(weight if ctx.needs_input_grad[0] else None, saved)
+        ctx.linear = (tuple(x.shape), x.dtype, weight.dtype, bias.dtype if bias is not None else None)
+        lead = (x.shape[1], x.shape[0]) if swap else x.shape[:-1]
+        y = y.view(*lead, weight.shape[0])
+        return y.transpose(0, 1) if swap else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        weight, saved = ctx.saved_tensors
+        xshape, dtype, wdtype, bdtype = ctx.linear
+        dx = dw = db = None
+        if ctx.needs_input_grad[0]:
+            swap = dy.dim() == 3 and not dy.is_contiguous() and dy.transpose(0, 1).is_contiguous()
+            g = (dy.transpose(0, 1) if swap else dy).reshape(-1, dy.shape[-1])
+            dx = g @ weight.to(dtype)
+            dx = dx.view(xshape[1], xshape[0], -1).transpose(0, 1) if swap else dx.view(xshape)
+        if ctx.saved8 is not None:
+            r = weight_grad8(dy, Checkpoint8(saved, *ctx.saved8), bias=bdtype is not None)
+            dw, db = r if bdtype is not None else (r, None)
+            dw = dw.to(wdtype) if ctx.needs_input_grad[1] else None
+            db = db.to(bdtype) if db is not None and ctx.needs_input_grad[2] else None
+        return dx, dw, db
+
+
+def linear8(x, weight, bias=None):
+    """``torch.nn.functional.linear`` that keeps its input in 8 bits for the backward pass: y and dx are the linear layer's,
+    dW (and db) come from ``weight_grad8``.  ``x`` [..., K] float32 / bfloat16 / float16; ``weight`` [N,K] and ``bias``
+    [N] in float32 (master parameters, rounded to x's type for the products) or in x's type, which is also their
+    gradients' type.  The in-projection in front of ``gated_scan``."""
+    _kind(x, "x")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise RuntimeError("x %s and weight %s do not fit" % (tuple(x.shape), tuple(weight.shape)))
+    for t, name, shape in ((weight, "weight", tuple(weight.shape)), (bias, "bias", (weight.shape[0],))):
+        if t is not None and (t.dtype not in (torch.float32, x.dtype) or t.device != x.device or tuple(t.shape) != shape):
+            raise RuntimeError("%s must be float32 or %s %s on %s" % (name, x.dtype, shape, x.device))
+    _need_device(x, "x")
+    return _Linear8.apply(x, weight, bias)

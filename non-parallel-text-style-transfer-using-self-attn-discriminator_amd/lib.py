@@ -12,7 +12,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SAD_LIB") or os.path.join(_HERE, "_native", "libsad.so")   # SAD_LIB: A/B builds
 
-SRC_IDS, SRC_F32, SRC_BF16 = 0, 1, 2
+SRC_IDS, SRC_F32, SRC_BF16, SRC_F16 = 0, 1, 2, 3
 
 WS_FIELDS = ("LENS", "NEED", "X", "G", "CS", "HS", "KK", "Q", "U", "CTX", "DZ", "DX", "DU", "DQ",
              "DHFIN", "DC", "ACCF", "DL", "DWA", "DSSUM", "ROWS", "NROWS", "SYNC", "DZX", "HX", "K1TILES", "K1SLABS", "GA")
@@ -22,7 +22,10 @@ EXPORTS = ("sad_version", "sad_last_error", "sad_padded_dims", "sad_packed_bytes
            "sad_workspace_bytes", "sad_workspace_field", "sad_pack_weights", "sad_forward",
            "sad_backward", "sad_param_grads_accumulate", "sad_prep", "sad_softemb_fwd", "sad_softemb_bwd", "sad_uses_half_gates",
            "sad_inproj_fwd", "sad_inproj_bwd", "sad_lstm_fwd", "sad_lstm_bwd", "sad_attnpool_fwd", "sad_attnpool_bwd", "sad_debug_set", "sad_forward_noalloc",
-           "sad_gumbel_st_step", "sad_gumbel_st_step_bwd", "sad_soft_finalize")
+           "sad_gumbel_st_step", "sad_gumbel_st_step_bwd", "sad_soft_finalize",
+           "sad_gated_scan_workspace_bytes", "sad_gated_scan_kept_bytes", "sad_gated_scan_codes_bytes", "sad_gated_scan_fwd",
+           "sad_gated_scan_bwd", "sad_gated_scan_step", "sad_checkpoint8_bytes", "sad_checkpoint8_save",
+           "sad_checkpoint8_restore", "sad_weight_grad8_workspace_bytes", "sad_weight_grad8")
 
 DBG_NO_PERSIST, DBG_SPIN_LIMIT, DBG_WITHHOLD_FWD, DBG_WITHHOLD_BWD, DBG_WITHHOLD_UPPER_ONLY, DBG_WGRAD_ATOMICS = 0, 1, 2, 3, 4, 5
 
@@ -95,6 +98,18 @@ class SadBwdArgs(ctypes.Structure):
     ]
 
 
+class SadScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int32), ("T", c_int32), ("D", c_int32), ("kind", c_int32), ("gated", c_int32), ("reverse", c_int32),
+        ("z", c_void_p), ("z_stride_b", c_int64), ("z_stride_t", c_int64),
+        ("lengths", c_void_p), ("h0", c_void_p),
+        ("y", c_void_p), ("y_stride_b", c_int64), ("y_stride_t", c_int64),
+        ("h_last", c_void_p), ("kept", c_void_p), ("codes", c_void_p),
+        ("dy", c_void_p), ("dy_stride_b", c_int64), ("dy_stride_t", c_int64), ("dh_last", c_void_p),
+        ("dz", c_void_p), ("dz_stride_b", c_int64), ("dz_stride_t", c_int64), ("dh0", c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -142,6 +157,21 @@ def load():
     lib.sad_gumbel_st_step_bwd.argtypes = [c_int32, c_int32, c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p, c_float,
                                            c_void_p, c_int64, c_void_p]
     lib.sad_soft_finalize.argtypes = [c_int32] * 8 + [c_void_p, c_int32, c_int64, c_int64] + [c_void_p] * 7
+    lib.sad_gated_scan_workspace_bytes.argtypes = [c_int32] * 3
+    lib.sad_gated_scan_kept_bytes.argtypes = [c_int32] * 3
+    lib.sad_gated_scan_codes_bytes.argtypes = [c_int32] * 4
+    lib.sad_gated_scan_fwd.argtypes = [POINTER(SadScanArgs), c_void_p, c_void_p]
+    lib.sad_gated_scan_bwd.argtypes = [POINTER(SadScanArgs), c_void_p, c_void_p]
+    lib.sad_gated_scan_step.argtypes = [c_int32] * 4 + [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                                        c_void_p, c_int64, c_void_p]
+    lib.sad_checkpoint8_bytes.argtypes = [c_int64] * 2
+    lib.sad_checkpoint8_save.argtypes = [c_int64] * 3 + [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p]
+    lib.sad_checkpoint8_restore.argtypes = [c_int64] * 2 + [c_int32, c_void_p, c_void_p, c_void_p]
+    lib.sad_weight_grad8_workspace_bytes.argtypes = [c_int64] * 3
+    lib.sad_weight_grad8.argtypes = [c_int64] * 4 + [c_int32, c_void_p, c_int64, c_int64] + [c_void_p] * 5
+    for name in ("sad_gated_scan_workspace_bytes", "sad_gated_scan_kept_bytes", "sad_gated_scan_codes_bytes",
+                 "sad_checkpoint8_bytes", "sad_weight_grad8_workspace_bytes"):
+        getattr(lib, name).restype = c_size_t
     for name in EXPORTS:
         getattr(lib, name)   # AttributeError here = header/library drift
     _lib = lib
