@@ -49,14 +49,24 @@ __device__ __forceinline__ unsigned c8_any_lost(unsigned w) {
     w ^= 0x80808080u;
     return (w - 0x01010101u) & ~w & 0x80808080u;
 }
-// code N of w times 2^e: exact
+// code N of w: one conversion with a sign-extended byte operand (from C++ the compiler makes two or three instructions)
 template <int N>
-__device__ __forceinline__ float c8_value(unsigned w, float scale) {
-    return (float)(signed char)(w >> (8 * N)) * scale;
+__device__ __forceinline__ float c8_int(unsigned w) {
+    float r;
+    if constexpr (N == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(r) : "v"(w));
+    if constexpr (N == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(r) : "v"(w));
+    if constexpr (N == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(r) : "v"(w));
+    if constexpr (N == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(r) : "v"(w));
+    return r;
 }
+// ... times 2^e: exact
+template <int N>
+__device__ __forceinline__ float c8_value(unsigned w, float scale) { return c8_int<N>(w) * scale; }
+template <int N>
+__device__ __forceinline__ bool c8_is_lost(unsigned w) { return ((w >> (8 * N)) & 0xffu) == C8_LOST; }
 template <int N>
 __device__ __forceinline__ float c8_value_checked(unsigned w, float scale) {
-    return ((w >> (8 * N)) & 0xffu) == C8_LOST ? __builtin_nanf("") : c8_value<N>(w, scale);
+    return c8_is_lost<N>(w) ? __builtin_nanf("") : c8_value<N>(w, scale);
 }
 
 // ---- element conversions ------------------------------------------------------------------------------------------

@@ -29,12 +29,14 @@ namespace sad {
 
 constexpr int SC_STEPS = 16;       // time steps of a block: states kept, loads in flight
 constexpr int SC_CH = 128;         // channels of a wave
+constexpr int SC_GROUP = 4;        // time chunks whose maps one workgroup joins
 constexpr float SC_LOG2E = 1.4426950408889634f;
 
 struct ScanP {
     int B, T, D, nblk, ncg;        // nblk = ceil(T / 16), ncg = ceil(D / 128)
     int reverse;
     int nchunk, cblk;              // time chunks per sentence, blocks per chunk
+    int group, ngroup;             // chunks of a group (waves of a summing workgroup), groups per sentence
     const void* z; long long z_sb, z_st;
     const int* lengths;
     const float* h0;
@@ -43,11 +45,13 @@ struct ScanP {
     float* kept;                   // [B][nblk][D]
     unsigned char* codes;          // [B][nblk][parts][D][16], steps in scan order
     unsigned char* exps;           // [B][nblk][parts][ceil(D/32)][16]
+    unsigned* lost;                // [B][nblk][ncg]: does a wave's block hold a lost (non-finite) entry
     const void* dy; long long dy_sb, dy_st;
     const float* dh_last;
     void* dz; long long dz_sb, dz_st;
     float* dh0;
-    float* sums;                   // [B][nchunk][2][D]: (M, v) of a chunk, chunks in the order of the walk
+    float* sums;                   // [B][nchunk][2][D]: (M, v) of the chunks of its group in front of a chunk, in the order of
+                                   // the walk; then [B][ngroup][2][D]: (M, v) of a group
 };
 
 // two neighbouring channels of one row
@@ -55,6 +59,13 @@ template <int KIND> struct Pair {
     typedef unsigned raw;
     static __device__ __forceinline__ raw load(const void* p) { return *(const u32h*)p; }
     static __device__ __forceinline__ raw zero() { return 0u; }
+    // magnitudes as ordered integers, the first non-finite one, and the float such an integer stands for
+    static constexpr unsigned nonfinite = KIND == SAD_SRC_BF16 ? 0x7f80u : 0x7c00u;
+    static __device__ __forceinline__ unsigned mag(raw r, int e) { return e == 0 ? r & 0x7fffu : (r >> 16) & 0x7fffu; }
+    static __device__ __forceinline__ float mag_value(unsigned m) {
+        if constexpr (KIND == SAD_SRC_BF16) return __builtin_bit_cast(float, m << 16);
+        else return (float)__builtin_bit_cast(_Float16, (unsigned short)m);
+    }
     static __device__ __forceinline__ f32x2 get(raw r) {
         if constexpr (KIND == SAD_SRC_BF16)
             return f32x2{__builtin_bit_cast(float, r << 16), __builtin_bit_cast(float, r & 0xffff0000u)};
@@ -76,36 +87,49 @@ template <> struct Pair<SAD_SRC_F32> {
     typedef f32x2 raw;
     static __device__ __forceinline__ raw load(const void* p) { return *(const f32x2u*)p; }
     static __device__ __forceinline__ raw zero() { return f32x2{0.f, 0.f}; }
+    static constexpr unsigned nonfinite = C8_NONFINITE;
+    static __device__ __forceinline__ unsigned mag(raw r, int e) { return c8_abs_bits(r[e]); }
+    static __device__ __forceinline__ float mag_value(unsigned m) { return __builtin_bit_cast(float, m); }
     static __device__ __forceinline__ f32x2 get(raw r) { return r; }
     static __device__ __forceinline__ void store(void* p, f32x2 v) { *(f32x2u*)p = v; }
 };
 
 // sigmoid(-f); exp2's overflow to infinity gives the limit 0
 __device__ __forceinline__ float sc_share(float f) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(SC_LOG2E * f)); }
-// p = sigmoid(v) is given together with q = 1 - p at full relative precision: u = e^-v, q = u p where q is the small one
-__device__ __forceinline__ void sc_gate(float v, float& p, float& q) {
-    const float u = __builtin_amdgcn_exp2f(-SC_LOG2E * v);
-    p = __builtin_amdgcn_rcpf(1.0f + u);
-    q = p > 0.5f ? u * p : 1.0f - p;
-}
+// u = 2^arg with arg kept where 1 + u and u / (1 + u) are finite; a NaN stays one (minimum, not min).  With arg = log2 e f:
+// 1 / (1 + u) = sigmoid(-f) and u / (1 + u) = sigmoid(f), each at full relative precision.
+__device__ __forceinline__ float sc_odds(float arg) { return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(arg, 126.0f)); }
 
 // position of a wave
 struct ScanAt {
     int b, cg, ord, cc, len, lo, hi;      // ord: chunk in the order of the walk; [lo, hi) its blocks
     bool valid;
 };
-// `backward`: the walk visits the chunks against the scan's direction
+// `backward`: the walk visits the chunks against the scan's direction.  A workgroup holds neighbouring channel groups, or,
+// where it sums, the chunks of one group.
+template <bool SUMS>
 __device__ __forceinline__ ScanAt scan_at(const ScanP& p, bool backward) {
     ScanAt w;
-    const int lane = threadIdx.x & 63;
-    const unsigned id = blockIdx.x * (blockDim.x >> 6) + (unsigned)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned per = (unsigned)p.ncg * p.nchunk;
-    w.b = (int)(id / per);
-    const unsigned r = id - (unsigned)w.b * per;
-    const int chunk = (int)(r / (unsigned)p.ncg);
-    w.cg = (int)(r - (unsigned)chunk * p.ncg);
-    w.valid = w.b < p.B;
-    w.ord = (p.reverse != 0) != backward ? p.nchunk - 1 - chunk : chunk;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned per, r;
+    if constexpr (SUMS) {
+        per = (unsigned)p.ncg * p.ngroup;
+        w.b = (int)(blockIdx.x / per);
+        r = blockIdx.x - (unsigned)w.b * per;
+        w.ord = (int)(r / (unsigned)p.ncg);
+        w.cg = (int)(r - (unsigned)w.ord * p.ncg);
+        w.ord = w.ord * p.group + wave;
+        w.valid = w.ord < p.nchunk;
+    } else {
+        const unsigned id = blockIdx.x * (blockDim.x >> 6) + (unsigned)wave;
+        per = (unsigned)p.ncg * p.nchunk;
+        w.b = (int)(id / per);
+        r = id - (unsigned)w.b * per;
+        w.ord = (int)(r / (unsigned)p.ncg);
+        w.cg = (int)(r - (unsigned)w.ord * p.ncg);
+        w.valid = w.b < p.B;
+    }
+    const int chunk = (p.reverse != 0) != backward ? p.nchunk - 1 - w.ord : w.ord;
     const int c0 = w.cg * SC_CH + 2 * lane;
     w.cc = c0 < p.D - 2 ? c0 : p.D - 2;
     w.lo = chunk * p.cblk;
@@ -119,68 +143,189 @@ __device__ __forceinline__ ScanAt scan_at(const ScanP& p, bool backward) {
     return w;
 }
 
-// (M, v) of every chunk in front of `ord` in the order of the walk, applied to the state h
+__device__ __forceinline__ void scan_apply(f32x2& h, f32x2 m, f32x2 v) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) h[e] = __builtin_fmaf(-m[e], h[e], h[e]) + v[e];
+}
+
+// The state that enters a chunk: the maps of the groups in front of its group, then of its predecessors in the group.
 __device__ __forceinline__ f32x2 scan_enter(const ScanP& p, const ScanAt& w, f32x2 h) {
-    const float* q = p.sums + (long long)w.b * p.nchunk * 2 * p.D + w.cc;
+    const long long D = p.D;
+    const int g = w.ord / p.group;
+    const float* q = p.sums + ((long long)p.B * p.nchunk + (long long)w.b * p.ngroup) * 2 * D + w.cc;
+    const float* l = p.sums + ((long long)w.b * p.nchunk + w.ord) * 2 * D + w.cc;
+    const f32x2 lm = *(const f32x2u*)l, lv = *(const f32x2u*)(l + D);
     int k = 0;
-    for (; k + 8 <= w.ord; k += 8) {
+    for (; k + 8 <= g; k += 8) {
         f32x2 m[8], v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            m[i] = *(const f32x2u*)(q + (long long)(k + i) * 2 * p.D);
-            v[i] = *(const f32x2u*)(q + (long long)(k + i) * 2 * p.D + p.D);
+            m[i] = *(const f32x2u*)(q + (k + i) * 2 * D);
+            v[i] = *(const f32x2u*)(q + (k + i) * 2 * D + D);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) h[e] = __builtin_fmaf(-m[i][e], h[e], h[e]) + v[i][e];
+        for (int i = 0; i < 8; ++i) scan_apply(h, m[i], v[i]);
     }
-    for (; k < w.ord; ++k) {
-        const f32x2 m = *(const f32x2u*)(q + (long long)k * 2 * p.D), v = *(const f32x2u*)(q + (long long)k * 2 * p.D + p.D);
+    if (k < g) {      // up to seven more; loads past the last group repeat it
+        f32x2 m[7], v[7];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) h[e] = __builtin_fmaf(-m[e], h[e], h[e]) + v[e];
+        for (int i = 0; i < 7; ++i) {
+            const int j = k + i < g ? k + i : g - 1;
+            m[i] = *(const f32x2u*)(q + j * 2 * D);
+            v[i] = *(const f32x2u*)(q + j * 2 * D + D);
+        }
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (k + i < g) scan_apply(h, m[i], v[i]);               // uniform
     }
+    scan_apply(h, lm, lv);
     return h;
 }
 
-// raw rows of one part of z (or of dy) in scan order; rows past the end of the tensor read the last one
-template <int KIND>
-__device__ __forceinline__ void sc_load_rows(typename Pair<KIND>::raw (&r)[SC_STEPS], const unsigned char* base, long long st, int kb,
-                                             int T, int reverse) {
+// End of a summing workgroup: every wave brings the map of its chunk, and leaves that of its predecessors in the group; the
+// last one leaves the whole group's.
+__device__ __forceinline__ void scan_leave(const ScanP& p, const ScanAt& w, f32x2 m, f32x2 v) {
+    __shared__ f32x2 maps[SC_GROUP][2][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    maps[wave][0][lane] = m;
+    maps[wave][1][lane] = v;
+    __syncthreads();
+    // composition: h -> h - (m1 + m2 - m1 m2) h + (v1 - m2 v1 + v2)
+    f32x2 pm{0.f, 0.f}, pv{0.f, 0.f};
+    auto then = [&](f32x2 m2, f32x2 v2) {
+        scan_apply(pv, m2, v2);
 #pragma unroll
-    for (int i = 0; i < SC_STEPS; ++i) {
-        const int t = kb * SC_STEPS + (reverse ? SC_STEPS - 1 - i : i);
-        r[i] = Pair<KIND>::load(base + (long long)(t < T ? t : T - 1) * st);
+        for (int e = 0; e < 2; ++e) pm[e] = __builtin_fmaf(m2[e], 1.0f - pm[e], pm[e]);
+    };
+    for (int k = 0; k < wave; ++k) then(maps[k][0][lane], maps[k][1][lane]);
+    if (w.valid) {
+        float* q = p.sums + ((long long)w.b * p.nchunk + w.ord) * 2 * p.D + w.cc;
+        *(f32x2u*)q = pm;
+        *(f32x2u*)(q + p.D) = pv;
+    }
+    if (wave == p.group - 1) {
+        then(m, v);
+        float* q = p.sums + ((long long)p.B * p.nchunk + (long long)w.b * p.ngroup + w.ord / p.group) * 2 * p.D + w.cc;
+        *(f32x2u*)q = pm;
+        *(f32x2u*)(q + p.D) = pv;
     }
 }
 
-// Codes of one row of one part: two values per lane, the 16 lanes of a DPP row share the exponent.
-// `in0` / `in1`: this lane's entry belongs to the 32 channels of its 16 lanes
-template <int KIND>
-__device__ __forceinline__ void sc_encode(f32x2 v, bool in0, bool in1, unsigned& u0, unsigned& u1, unsigned& byte) {
-    const unsigned b0 = in0 ? c8_abs_bits(v[0]) : 0u, b1 = in1 ? c8_abs_bits(v[1]) : 0u;
-    auto row_max = [](unsigned m) {
-        auto ror = [](unsigned x, auto c) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, decltype(c)::value, 0xf, 0xf, false); };
-        unsigned t;
-        t = ror(m, std::integral_constant<int, 0x128>{}); m = m > t ? m : t;      // row_ror:8
-        t = ror(m, std::integral_constant<int, 0x124>{}); m = m > t ? m : t;
-        t = ror(m, std::integral_constant<int, 0x122>{}); m = m > t ? m : t;
-        t = ror(m, std::integral_constant<int, 0x121>{}); m = m > t ? m : t;
-        return m;
-    };
-    unsigned top = row_max(b0 > b1 ? b0 : b1);
-    const bool bad = __any(top >= C8_NONFINITE);
-    if (bad) top = row_max((b0 < C8_NONFINITE ? b0 : 0u) > (b1 < C8_NONFINITE ? b1 : 0u) ? (b0 < C8_NONFINITE ? b0 : 0u)
-                                                                                         : (b1 < C8_NONFINITE ? b1 : 0u));
-    const int e = c8_exponent<KIND>(top);
-    const float inv = c8_inv_scale(e), cap = e == C8Range<KIND>::hi + 127 ? 63.f : 127.f;
-    u0 = c8_code(v[0], inv, cap);
-    u1 = c8_code(v[1], inv, cap);
-    if (bad) {
-        if (c8_abs_bits(v[0]) >= C8_NONFINITE) u0 = C8_LOST;
-        if (c8_abs_bits(v[1]) >= C8_NONFINITE) u1 = C8_LOST;
+// A lane's 32-bit offset, opaque from here on: its zero extension then stays in the block of code that uses it, where
+// scalar base + lane offset is one address operand; hoisted out of a loop it costs a 64-bit vector addition per access.
+__device__ __forceinline__ unsigned sc_here(unsigned v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// Walk over the 16 rows of a block in scan order.  The row pointer is uniform (scalar registers), a lane adds its own
+// 32-bit offset; rows past the end of the tensor repeat the last one.
+struct RowWalk {
+    const unsigned char* p;
+    long long step;
+    int t, dt, last;
+    __device__ __forceinline__ RowWalk(const void* base, long long st, int kb, int T, int reverse) {
+        t = kb * SC_STEPS + (reverse ? SC_STEPS - 1 : 0);
+        dt = reverse ? -1 : 1;
+        last = T - 1;
+        step = reverse ? -st : st;
+        p = (const unsigned char*)base + (long long)(t < T ? t : T - 1) * st;
     }
-    byte = (unsigned)e;
+    __device__ __forceinline__ void next() {
+        const bool move = dt < 0 ? t <= last : t < last;
+        p += move ? step : 0;
+        t += dt;
+    }
+};
+
+template <int KIND, int Q0, int Q1, int PARTS>
+__device__ __forceinline__ void sc_load_rows(typename Pair<KIND>::raw (&r)[PARTS][SC_STEPS], const void* base, long long st,
+                                             const unsigned (&voff)[PARTS], int kb, int T, int reverse) {
+    RowWalk w(base, st, kb, T, reverse);
+    unsigned v[PARTS];
+#pragma unroll
+    for (int q = Q0; q < Q1; ++q) v[q] = sc_here(voff[q]);
+#pragma unroll
+    for (int i = 0; i < SC_STEPS; ++i) {
+#pragma unroll
+        for (int q = Q0; q < Q1; ++q) r[q][i] = Pair<KIND>::load(w.p + v[q]);
+        w.next();
+    }
+}
+
+// Largest of m[i] over the 16 lanes of a DPP row, for all 16 steps i at once: lane l gets the one of step l & 15.  Each
+// level hands half of the steps to a partner lane and keeps the other half; the partners l^8, l^7, l^2, l^1 are the DPP
+// controls row_ror:8, row_half_mirror and two quad permutations, and together reach every lane of the row.
+__device__ __forceinline__ unsigned sc_row_max16(const unsigned (&m)[SC_STEPS], int lane) {
+    auto meet = [](unsigned keep, unsigned send, auto ctrl) {
+        const unsigned got = (unsigned)__builtin_amdgcn_update_dpp(0, (int)send, decltype(ctrl)::value, 0xf, 0xf, false);
+        return keep > got ? keep : got;
+    };
+    unsigned a[8], b[4], c[2];
+    const bool h8 = lane & 8, h4 = lane & 4, h2 = lane & 2, h1 = lane & 1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = meet(h8 ? m[k + 8] : m[k], h8 ? m[k] : m[k + 8], std::integral_constant<int, 0x128>{});
+#pragma unroll
+    for (int k = 0; k < 4; ++k) b[k] = meet(h4 ? a[k + 4] : a[k], h4 ? a[k] : a[k + 4], std::integral_constant<int, 0x141>{});
+#pragma unroll
+    for (int k = 0; k < 2; ++k) c[k] = meet(h2 ? b[k + 2] : b[k], h2 ? b[k] : b[k + 2], std::integral_constant<int, 0x4E>{});
+    return meet(h1 ? c[1] : c[0], h1 ? c[0] : c[1], std::integral_constant<int, 0xB1>{});
+}
+
+// Codes of one part of a block: 16 steps of this lane's two channels, whose 16-lane row shares an exponent per step.
+// in0 / in1: the lane's entry belongs to the 32 channels of its row.  code[e][j]: steps 4j .. 4j+3 of channel cc + e;
+// `byte`: exponent of step lane & 15.  Returns whether an entry of the wave was lost.
+template <int KIND>
+__device__ __forceinline__ bool sc_encode(const typename Pair<KIND>::raw (&r)[SC_STEPS], bool in0, bool in1, int lane,
+                                          unsigned (&code)[2][4], unsigned& byte) {
+    typedef Pair<KIND> P;
+    unsigned m[SC_STEPS];
+#pragma unroll
+    for (int i = 0; i < SC_STEPS; ++i) {
+        const unsigned m0 = in0 ? P::mag(r[i], 0) : 0u, m1 = in1 ? P::mag(r[i], 1) : 0u;
+        m[i] = m0 > m1 ? m0 : m1;
+    }
+    unsigned top = sc_row_max16(m, lane);
+    const bool lost = __any(top >= P::nonfinite);
+    if (lost) {
+#pragma unroll
+        for (int i = 0; i < SC_STEPS; ++i) {
+            const unsigned m0 = in0 && P::mag(r[i], 0) < P::nonfinite ? P::mag(r[i], 0) : 0u;
+            const unsigned m1 = in1 && P::mag(r[i], 1) < P::nonfinite ? P::mag(r[i], 1) : 0u;
+            m[i] = m0 > m1 ? m0 : m1;
+        }
+        top = sc_row_max16(m, lane);
+    }
+    const int ex = c8_exponent<KIND>(__builtin_bit_cast(unsigned, P::mag_value(top)));
+    byte = (unsigned)ex;
+    const float inv = c8_inv_scale(ex);
+    const bool rare = lost || __any(ex == C8Range<KIND>::hi + 127);
+    unsigned u[2][SC_STEPS];
+    static_for<SC_STEPS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        // the exponent's reciprocal of step i from lane i of the row (row_newbcast)
+        const float q = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, inv), 0x150 + i, 0xf, 0xf, false));
+        const f32x2 v = P::get(r[i]);
+        // x * 2^-e + 1.5 * 2^23: the sum's step is 1, so the one rounding is the code's (ties to even), and the low byte
+        // of its bits is the code
+#pragma unroll
+        for (int e = 0; e < 2; ++e) u[e][i] = __builtin_bit_cast(unsigned, __builtin_fmaf(v[e], q, 12582912.0f));
+        if (rare) {
+            const float cap = q == c8_inv_scale(C8Range<KIND>::hi + 127) ? 63.f : 127.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) u[e][i] = P::mag(r[i], e) >= P::nonfinite ? C8_LOST : c8_code(v[e], q, cap);
+        }
+    });
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // v_perm_b32: selectors 0-3 take the second operand's bytes, 4-7 the first one's
+            const unsigned lo = __builtin_amdgcn_perm(u[e][4 * j + 1], u[e][4 * j], 0x0c0c0400u);
+            const unsigned hi = __builtin_amdgcn_perm(u[e][4 * j + 3], u[e][4 * j + 2], 0x04000c0cu);
+            code[e][j] = lo | hi;
+        }
+    return lost;
 }
 
 // Forward.  SAVE: 0 nothing, 1 the state entering each block, 2 that and the 8-bit codes of z.
@@ -188,121 +333,104 @@ template <int KIND, bool GATED, int SAVE>
 __global__ __launch_bounds__(256) void k_scan_fwd(ScanP p) {
     typedef typename Pair<KIND>::raw raw;
     constexpr int PARTS = GATED ? 3 : 2, EB = Elem<KIND>::bytes;
-    const ScanAt w = scan_at(p, false);
+    const ScanAt w = scan_at<false>(p, false);
     if (!w.valid) return;
     const int lane = threadIdx.x & 63;
     const long long zst = p.z_st * EB, yst = p.y_st * EB;
-    const unsigned char* zx = (const unsigned char*)p.z + (w.b * p.z_sb + w.cc) * EB;
-    const unsigned char* zf = zx + (long long)p.D * EB;
-    const unsigned char* zo = zf + (long long)p.D * EB;
-    unsigned char* yp = (unsigned char*)p.y + (w.b * p.y_sb + w.cc) * EB;
+    const unsigned char* zb = (const unsigned char*)p.z + w.b * p.z_sb * EB;
+    unsigned char* yb = (unsigned char*)p.y + w.b * p.y_sb * EB;
+    unsigned voff[PARTS];
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) voff[q] = (unsigned)(q * p.D + w.cc) * EB;
     const int vhi = (w.len + SC_STEPS - 1) / SC_STEPS, hi = w.hi < vhi ? w.hi : vhi;     // blocks that hold a valid step
     for (int kb = hi > w.lo ? hi : w.lo; kb < w.hi; ++kb)                                 // blocks behind the sentence
         for (int i = 0; i < SC_STEPS; ++i)
-            if (kb * SC_STEPS + i < p.T) Pair<KIND>::store(yp + (long long)(kb * SC_STEPS + i) * yst, f32x2{0.f, 0.f});
+            if (kb * SC_STEPS + i < p.T) Pair<KIND>::store(yb + (long long)(kb * SC_STEPS + i) * yst + voff[0], f32x2{0.f, 0.f});
     f32x2 h = p.h0 != nullptr ? (f32x2)*(const f32x2u*)(p.h0 + (long long)w.b * p.D + w.cc) : f32x2{0.f, 0.f};
-    if (p.nchunk > 1) h = scan_enter(p, w, h);
-
     const int c0 = w.cg * SC_CH + 2 * lane;
     const bool own0 = c0 < p.D && w.cc == c0, own1 = c0 < p.D;      // the lane's own channels among (cc, cc + 1)
-    raw nx[SC_STEPS], nf[SC_STEPS], no[SC_STEPS];
-    auto issue = [&](int kb) {
-        sc_load_rows<KIND>(nx, zx, zst, kb, p.T, p.reverse);
-        sc_load_rows<KIND>(nf, zf, zst, kb, p.T, p.reverse);
-        if constexpr (GATED) sc_load_rows<KIND>(no, zo, zst, kb, p.T, p.reverse);
-    };
+    raw nz[PARTS][SC_STEPS];
     const int n = hi - w.lo;
-    if (n > 0) issue(p.reverse ? hi - 1 : w.lo);
+    if (n > 0) sc_load_rows<KIND, 0, PARTS>(nz, zb, zst, voff, p.reverse ? hi - 1 : w.lo, p.T, p.reverse);
+    if (p.nchunk > 1) h = scan_enter(p, w, h);
     for (int it = 0; it < n; ++it) {
         const int kb = p.reverse ? hi - 1 - it : w.lo + it;
-        raw x[SC_STEPS], f[SC_STEPS], o[SC_STEPS];
+        raw z[PARTS][SC_STEPS];
 #pragma unroll
-        for (int i = 0; i < SC_STEPS; ++i) {
-            x[i] = nx[i];
-            f[i] = nf[i];
-            if constexpr (GATED) o[i] = no[i];
-        }
-        if (it + 1 < n) issue(p.reverse ? kb - 1 : kb + 1);
+        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+            for (int i = 0; i < SC_STEPS; ++i) z[q][i] = nz[q][i];
+        if (it + 1 < n) sc_load_rows<KIND, 0, PARTS>(nz, zb, zst, voff, p.reverse ? kb - 1 : kb + 1, p.T, p.reverse);
         if constexpr (SAVE > 0) *(f32x2u*)(p.kept + ((long long)w.b * p.nblk + kb) * p.D + w.cc) = h;
-        unsigned code[SAVE == 2 ? PARTS : 1][2][4], eb[SAVE == 2 ? PARTS : 1][4];
+        if constexpr (SAVE == 2) {
+            const int nb = (p.D + C8_BLOCK - 1) / C8_BLOCK;
+            const long long tile = ((long long)w.b * p.nblk + kb) * PARTS;
+            bool lost = false;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                unsigned code[2][4], byte;
+                lost |= sc_encode<KIND>(z[q], own0, own1, lane, code, byte);
+                unsigned char* cp = p.codes + ((tile + q) * p.D + w.cc) * SC_STEPS;
+                if (own0) *(u32x4*)cp = u32x4{code[0][0], code[0][1], code[0][2], code[0][3]};
+                if (own1) *(u32x4*)(cp + SC_STEPS) = u32x4{code[1][0], code[1][1], code[1][2], code[1][3]};
+                const int blk = (w.cg * SC_CH + (lane & 48) * 2) / C8_BLOCK;
+                if (blk < nb) p.exps[((tile + q) * nb + blk) * SC_STEPS + (lane & 15)] = (unsigned char)byte;
+            }
+            if (lane == 0) p.lost[((long long)w.b * p.nblk + kb) * p.ncg + w.cg] = lost ? 1u : 0u;
+        }
         auto block = [&](auto full) {
+            unsigned char* yr = yb + (long long)(kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 : 0)) * yst;
+            const unsigned vy = sc_here(voff[0]);
 #pragma unroll
             for (int i = 0; i < SC_STEPS; ++i) {
                 const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
                 const bool ok = decltype(full)::value || t < w.len;
-                const f32x2 xv = Pair<KIND>::get(x[i]), fv = Pair<KIND>::get(f[i]);
-                f32x2 hn, ov;
+                const f32x2 xv = Pair<KIND>::get(z[0][i]), fv = Pair<KIND>::get(z[1][i]);
+                f32x2 hn;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) hn[e] = __builtin_fmaf(sc_share(fv[e]), xv[e] - h[e], h[e]);
                 if (ok) h = hn;                                     // uniform
                 f32x2 yv = h;
                 if constexpr (GATED) {
-                    ov = Pair<KIND>::get(o[i]);
+                    const f32x2 ov = Pair<KIND>::get(z[PARTS - 1][i]);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) yv[e] = h[e] * sigmoidf_(ov[e]);
                 }
                 if (!ok) yv = f32x2{0.f, 0.f};
-                if (decltype(full)::value || t < p.T) Pair<KIND>::store(yp + (long long)t * yst, yv);
-                if constexpr (SAVE == 2) {
-                    unsigned u0, u1, e;
-                    auto put = [&](int q, f32x2 v) {
-                        sc_encode<KIND>(v, own0, own1, u0, u1, e);
-                        const int sh = 8 * (i & 3);
-                        if ((i & 3) == 0) { code[q][0][i >> 2] = u0; code[q][1][i >> 2] = u1; eb[q][i >> 2] = e; }
-                        else { code[q][0][i >> 2] |= u0 << sh; code[q][1][i >> 2] |= u1 << sh; eb[q][i >> 2] |= e << sh; }
-                    };
-                    put(0, xv);
-                    put(1, fv);
-                    if constexpr (GATED) put(2, ov);
-                }
+                if (decltype(full)::value || t < p.T) Pair<KIND>::store(yr + vy, yv);
+                yr += p.reverse ? -yst : yst;
             }
         };
         if ((kb + 1) * SC_STEPS <= w.len) block(std::integral_constant<bool, true>{});
         else block(std::integral_constant<bool, false>{});
-        if constexpr (SAVE == 2) {
-            const int nb = (p.D + C8_BLOCK - 1) / C8_BLOCK;
-            const long long tile = ((long long)w.b * p.nblk + kb) * PARTS;
-#pragma unroll
-            for (int q = 0; q < PARTS; ++q) {
-                unsigned char* cp = p.codes + ((tile + q) * p.D + w.cc) * SC_STEPS;
-                if (own0) *(u32x4*)cp = u32x4{code[q][0][0], code[q][0][1], code[q][0][2], code[q][0][3]};
-                if (own1) *(u32x4*)(cp + SC_STEPS) = u32x4{code[q][1][0], code[q][1][1], code[q][1][2], code[q][1][3]};
-                if ((lane & 15) == 0 && own1)
-                    *(u32x4*)(p.exps + ((tile + q) * nb + c0 / C8_BLOCK) * SC_STEPS) = u32x4{eb[q][0], eb[q][1], eb[q][2], eb[q][3]};
-            }
-        }
     }
     if (w.ord == p.nchunk - 1) *(f32x2u*)(p.h_last + (long long)w.b * p.D + w.cc) = h;
 }
 
 // (M, v) of one chunk, forward: the chunk's steps from the zero state.
 template <int KIND>
-__global__ __launch_bounds__(256) void k_scan_sum(ScanP p) {
+__global__ __launch_bounds__(64 * SC_GROUP) void k_scan_sum(ScanP p) {
     typedef typename Pair<KIND>::raw raw;
     constexpr int EB = Elem<KIND>::bytes;
-    const ScanAt w = scan_at(p, false);
-    if (!w.valid || w.ord == p.nchunk - 1) return;                  // the last chunk's map is not needed
+    const ScanAt w = scan_at<true>(p, false);
     const long long zst = p.z_st * EB;
-    const unsigned char* zx = (const unsigned char*)p.z + (w.b * p.z_sb + w.cc) * EB;
-    const unsigned char* zf = zx + (long long)p.D * EB;
-    const int vhi = (w.len + SC_STEPS - 1) / SC_STEPS, hi = w.hi < vhi ? w.hi : vhi, n = hi - w.lo;
+    const unsigned char* zb = (const unsigned char*)p.z + w.b * p.z_sb * EB;
+    const unsigned voff[2] = {(unsigned)w.cc * EB, (unsigned)(p.D + w.cc) * EB};
+    const int vhi = (w.len + SC_STEPS - 1) / SC_STEPS, hi = w.hi < vhi ? w.hi : vhi;
+    const int n = w.ord < p.nchunk - 1 ? hi - w.lo : 0;             // nothing follows the last chunk's map
     f32x2 h{0.f, 0.f}, m{0.f, 0.f};
-    raw nx[SC_STEPS], nf[SC_STEPS];
-    auto issue = [&](int kb) {
-        sc_load_rows<KIND>(nx, zx, zst, kb, p.T, p.reverse);
-        sc_load_rows<KIND>(nf, zf, zst, kb, p.T, p.reverse);
-    };
-    if (n > 0) issue(p.reverse ? hi - 1 : w.lo);
+    raw nz[2][SC_STEPS];
+    if (n > 0) sc_load_rows<KIND, 0, 2>(nz, zb, zst, voff, p.reverse ? hi - 1 : w.lo, p.T, p.reverse);
     for (int it = 0; it < n; ++it) {
         const int kb = p.reverse ? hi - 1 - it : w.lo + it;
-        raw x[SC_STEPS], f[SC_STEPS];
+        raw z[2][SC_STEPS];
 #pragma unroll
-        for (int i = 0; i < SC_STEPS; ++i) { x[i] = nx[i]; f[i] = nf[i]; }
-        if (it + 1 < n) issue(p.reverse ? kb - 1 : kb + 1);
+        for (int i = 0; i < SC_STEPS; ++i) { z[0][i] = nz[0][i]; z[1][i] = nz[1][i]; }
+        if (it + 1 < n) sc_load_rows<KIND, 0, 2>(nz, zb, zst, voff, p.reverse ? kb - 1 : kb + 1, p.T, p.reverse);
 #pragma unroll
         for (int i = 0; i < SC_STEPS; ++i) {
             const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-            const f32x2 xv = Pair<KIND>::get(x[i]), fv = Pair<KIND>::get(f[i]);
+            const f32x2 xv = Pair<KIND>::get(z[0][i]), fv = Pair<KIND>::get(z[1][i]);
             if (t < w.len) {                                        // uniform
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -313,41 +441,83 @@ __global__ __launch_bounds__(256) void k_scan_sum(ScanP p) {
             }
         }
     }
-    float* q = p.sums + ((long long)w.b * p.nchunk + w.ord) * 2 * p.D + w.cc;
-    *(f32x2u*)q = m;
-    *(f32x2u*)(q + p.D) = h;
+    scan_leave(p, w, m, h);
 }
 
-// What a block of the backward pass reads of z: the rows themselves, or codes and exponents.
+// What a block of the backward pass reads of z (parts Q0 ..): the rows themselves, or codes and exponents.
 template <int KIND, int PARTS, bool CODES> struct ScanIn;
 template <int KIND, int PARTS> struct ScanIn<KIND, PARTS, false> {
     typename Pair<KIND>::raw r[PARTS][SC_STEPS];
-    template <int Q> __device__ __forceinline__ void load(const ScanP& p, const ScanAt& w, int kb) {
-        sc_load_rows<KIND>(r[Q], (const unsigned char*)p.z + (w.b * p.z_sb + w.cc + (long long)Q * p.D) * Elem<KIND>::bytes,
-                           p.z_st * Elem<KIND>::bytes, kb, p.T, p.reverse);
+    template <int Q0, int Q1> __device__ __forceinline__ void load(const ScanP& p, const ScanAt& w, int kb) {
+        constexpr int EB = Elem<KIND>::bytes;
+        unsigned voff[PARTS];
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) voff[q] = (unsigned)(q * p.D + w.cc) * EB;
+        sc_load_rows<KIND, Q0, Q1>(r, (const unsigned char*)p.z + w.b * p.z_sb * EB, p.z_st * EB, voff, kb, p.T, p.reverse);
     }
-    template <int Q, int I> __device__ __forceinline__ f32x2 get() const { return Pair<KIND>::get(r[Q][I]); }
+    __device__ __forceinline__ bool lost() const { return false; }
+    // makes the compiler decode x and f again instead of keeping 64 decoded registers alive between two uses
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < SC_STEPS; ++i) asm volatile("" : "+v"(r[q][i]));
+    }
+    // c times part Q of step I, and x of step I less h
+    template <int Q, int I, bool CHECKED> __device__ __forceinline__ f32x2 times(float c) const {
+        const f32x2 v = Pair<KIND>::get(r[Q][I]);
+        return f32x2{c * v[0], c * v[1]};
+    }
+    template <int I, bool CHECKED> __device__ __forceinline__ f32x2 x_less(f32x2 h) const {
+        const f32x2 v = Pair<KIND>::get(r[0][I]);
+        return f32x2{v[0] - h[0], v[1] - h[1]};
+    }
 };
 template <int KIND, int PARTS> struct ScanIn<KIND, PARTS, true> {
     u32x4 c[PARTS][2], e[PARTS][2];
-    template <int Q> __device__ __forceinline__ void load(const ScanP& p, const ScanAt& w, int kb) {
+    unsigned flag;
+    template <int Q0, int Q1> __device__ __forceinline__ void load(const ScanP& p, const ScanAt& w, int kb) {
         const int nb = (p.D + C8_BLOCK - 1) / C8_BLOCK;
-        const long long tile = ((long long)w.b * p.nblk + kb) * PARTS + Q;
-        const unsigned char* cp = p.codes + (tile * p.D + w.cc) * SC_STEPS;
-        c[Q][0] = *(const u32x4*)cp;
-        c[Q][1] = *(const u32x4*)(cp + SC_STEPS);
-        const unsigned char* ep = p.exps + tile * nb * SC_STEPS;
-        e[Q][1] = *(const u32x4*)(ep + (long long)((w.cc + 1) / C8_BLOCK) * SC_STEPS);
-        e[Q][0] = e[Q][1];
-        // channels D-2 and D-1 of the last lanes lie in different blocks of 32
-        if (p.D % C8_BLOCK == 1) e[Q][0] = *(const u32x4*)(ep + (long long)(w.cc / C8_BLOCK) * SC_STEPS);
+        const long long blk = (long long)w.b * p.nblk + kb;
+        if (Q0 < 2) flag = p.lost[blk * p.ncg + w.cg];
+#pragma unroll
+        for (int q = Q0; q < Q1; ++q) {
+            const long long tile = blk * PARTS + q;
+            const unsigned char* cp = p.codes + tile * p.D * SC_STEPS;
+            c[q][0] = *(const u32x4*)(cp + (unsigned)w.cc * SC_STEPS);
+            c[q][1] = *(const u32x4*)(cp + (unsigned)(w.cc + 1) * SC_STEPS);
+            const unsigned char* ep = p.exps + tile * nb * SC_STEPS;
+            e[q][1] = *(const u32x4*)(ep + (unsigned)((w.cc + 1) / C8_BLOCK) * SC_STEPS);
+            e[q][0] = e[q][1];
+            // channels D-2 and D-1 of the last lanes lie in different blocks of 32
+            if (p.D % C8_BLOCK == 1) e[q][0] = *(const u32x4*)(ep + (unsigned)(w.cc / C8_BLOCK) * SC_STEPS);
+        }
     }
-    template <int Q, int I> __device__ __forceinline__ f32x2 get() const {
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) asm volatile("" : "+v"(c[q][k]), "+v"(e[q][k]));
+    }
+    __device__ __forceinline__ bool lost() const { return __builtin_amdgcn_readfirstlane(flag) != 0; }
+    template <int Q, int I> __device__ __forceinline__ float scale(int k) const {
+        return c8_scale((e[Q][k][I >> 2] >> (8 * (I & 3))) & 0xffu);
+    }
+    template <int Q, int I, bool CHECKED> __device__ __forceinline__ f32x2 times(float f) const {
         f32x2 v;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const float scale = c8_scale((e[Q][k][I >> 2] >> (8 * (I & 3))) & 0xffu);
-            v[k] = c8_value_checked<I & 3>(c[Q][k][I >> 2], scale);
+            v[k] = c8_int<I & 3>(c[Q][k][I >> 2]) * (scale<Q, I>(k) * f);       // the power of two moves freely: one rounding
+            if (CHECKED && c8_is_lost<I & 3>(c[Q][k][I >> 2])) v[k] = __builtin_nanf("");
+        }
+        return v;
+    }
+    template <int I, bool CHECKED> __device__ __forceinline__ f32x2 x_less(f32x2 h) const {
+        f32x2 v;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            v[k] = __builtin_fmaf(c8_int<I & 3>(c[0][k][I >> 2]), scale<0, I>(k), -h[k]);
+            if (CHECKED && c8_is_lost<I & 3>(c[0][k][I >> 2])) v[k] = __builtin_nanf("");
         }
         return v;
     }
@@ -355,125 +525,136 @@ template <int KIND, int PARTS> struct ScanIn<KIND, PARTS, true> {
 
 // Backward.
 template <int KIND, bool GATED, bool CODES>
-__global__ __launch_bounds__(256) void k_scan_bwd(ScanP p) {
+__global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanP p) {
     typedef typename Pair<KIND>::raw raw;
     constexpr int PARTS = GATED ? 3 : 2, EB = Elem<KIND>::bytes;
-    const ScanAt w = scan_at(p, true);
+    const ScanAt w = scan_at<false>(p, true);
     if (!w.valid) return;
     const long long dyst = p.dy_st * EB, dzst = p.dz_st * EB;
-    const unsigned char* dyp = (const unsigned char*)p.dy + (w.b * p.dy_sb + w.cc) * EB;
-    unsigned char* gx = (unsigned char*)p.dz + (w.b * p.dz_sb + w.cc) * EB;
-    unsigned char* gf = gx + (long long)p.D * EB;
-    unsigned char* go = gf + (long long)p.D * EB;
+    const unsigned char* dyb = (const unsigned char*)p.dy + w.b * p.dy_sb * EB;
+    unsigned char* gb = (unsigned char*)p.dz + w.b * p.dz_sb * EB;
+    unsigned voff[PARTS];
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) voff[q] = (unsigned)(q * p.D + w.cc) * EB;
+    const unsigned dyoff[1] = {voff[0]};
     const int vhi = (w.len + SC_STEPS - 1) / SC_STEPS, hi = w.hi < vhi ? w.hi : vhi, n = hi - w.lo;
     for (int kb = hi > w.lo ? hi : w.lo; kb < w.hi; ++kb)
-        for (int i = 0; i < SC_STEPS; ++i) {
-            const int t = kb * SC_STEPS + i;
-            if (t < p.T) {
-                Pair<KIND>::store(gx + t * dzst, f32x2{0.f, 0.f});
-                Pair<KIND>::store(gf + t * dzst, f32x2{0.f, 0.f});
-                if constexpr (GATED) Pair<KIND>::store(go + t * dzst, f32x2{0.f, 0.f});
+        for (int i = 0; i < SC_STEPS; ++i)
+            if (kb * SC_STEPS + i < p.T) {
+#pragma unroll
+                for (int q = 0; q < PARTS; ++q) Pair<KIND>::store(gb + (long long)(kb * SC_STEPS + i) * dzst + voff[q], f32x2{0.f, 0.f});
             }
-        }
     f32x2 carry = p.dh_last != nullptr ? (f32x2)*(const f32x2u*)(p.dh_last + (long long)w.b * p.D + w.cc) : f32x2{0.f, 0.f};
-    if (p.nchunk > 1) carry = scan_enter(p, w, carry);
 
-    ScanIn<KIND, PARTS, CODES> nin;
-    raw ndy[SC_STEPS];
-    f32x2 nh;
+    // x, f and the kept state of the next block are loaded behind the states of this one, o and dy of this block in front of
+    // them: each load has one of the two passes over the block to arrive in, and at most 96 registers hold rows.
+    ScanIn<KIND, PARTS, CODES> in, nin;
+    f32x2 enter, nh;
     auto issue = [&](int kb) {
         nh = *(const f32x2u*)(p.kept + ((long long)w.b * p.nblk + kb) * p.D + w.cc);
-        nin.template load<0>(p, w, kb);
-        nin.template load<1>(p, w, kb);
-        if constexpr (GATED) nin.template load<2>(p, w, kb);
-        if (p.dy != nullptr) sc_load_rows<KIND>(ndy, dyp, dyst, kb, p.T, p.reverse);
-        else {
-#pragma unroll
-            for (int i = 0; i < SC_STEPS; ++i) ndy[i] = Pair<KIND>::zero();
-        }
+        nin.template load<0, 2>(p, w, kb);
     };
     if (n > 0) issue(p.reverse ? w.lo : hi - 1);
+    if (p.nchunk > 1) carry = scan_enter(p, w, carry);
     for (int it = 0; it < n; ++it) {
         const int kb = p.reverse ? w.lo + it : hi - 1 - it;
-        const ScanIn<KIND, PARTS, CODES> in = nin;
-        const f32x2 enter = nh;
-        raw dy[SC_STEPS];
+        raw dy[1][SC_STEPS];
+        in = nin;
+        enter = nh;
+        if constexpr (GATED) in.template load<2, PARTS>(p, w, kb);
+        if (p.dy != nullptr) sc_load_rows<KIND, 0, 1>(dy, dyb, dyst, dyoff, kb, p.T, p.reverse);
+        else {
 #pragma unroll
-        for (int i = 0; i < SC_STEPS; ++i) dy[i] = ndy[i];
-        if (it + 1 < n) issue(p.reverse ? kb + 1 : kb - 1);
-        auto block = [&](auto full) {
-            f32x2 h[SC_STEPS], s[SC_STEPS];
+            for (int i = 0; i < SC_STEPS; ++i) dy[0][i] = Pair<KIND>::zero();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const bool full_block = (kb + 1) * SC_STEPS <= w.len && !in.lost();
+        f32x2 h[SC_STEPS], odds[SC_STEPS];                          // states; e^f
+        auto states = [&](auto full) {
+            constexpr bool FULL = decltype(full)::value;
             f32x2 hc = enter;
             static_for<SC_STEPS>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-                const f32x2 xv = in.template get<0, i>(), fv = in.template get<1, i>();
+                const f32x2 fa = in.template times<1, i, !FULL>(SC_LOG2E), xd = in.template x_less<i, !FULL>(hc);
                 f32x2 hn;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    s[i][e] = sc_share(fv[e]);
-                    hn[e] = __builtin_fmaf(s[i][e], xv[e] - hc[e], hc[e]);
+                    odds[i][e] = sc_odds(fa[e]);
+                    hn[e] = __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + odds[i][e]), xd[e], hc[e]);
                 }
-                if (decltype(full)::value || t < w.len) hc = hn;    // uniform
+                if (FULL || t < w.len) hc = hn;                     // uniform
                 h[i] = hc;
             });
+        };
+        auto grads = [&](auto full) {
+            constexpr bool FULL = decltype(full)::value;
+            unsigned char* gr = gb + (long long)(kb * SC_STEPS + (p.reverse ? 0 : SC_STEPS - 1)) * dzst;
+            unsigned vg[PARTS];
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) vg[q] = sc_here(voff[q]);
             static_for<SC_STEPS>([&](auto jc) {
                 constexpr int i = SC_STEPS - 1 - decltype(jc)::value;
                 const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-                const bool ok = decltype(full)::value || t < w.len;
-                const f32x2 xv = in.template get<0, i>(), fv = in.template get<1, i>(), dyv = Pair<KIND>::get(dy[i]);
-                f32x2 dx, df, dov, cn;
+                const bool ok = FULL || t < w.len;
+                const f32x2 hp = i == 0 ? enter : h[i == 0 ? 0 : i - 1], dyv = Pair<KIND>::get(dy[0][i]);
+                const f32x2 xd = in.template x_less<i, !FULL>(hp);
+                f32x2 oa, dx, df, dov, cn;
+                if constexpr (GATED) oa = in.template times<PARTS - 1, i, !FULL>(-SC_LOG2E);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float hp = i == 0 ? enter[e] : h[i == 0 ? 0 : i - 1][e];
                     float dh = dyv[e];
                     if constexpr (GATED) {
-                        float so, sq;
-                        sc_gate(in.template get<2, i>()[e], so, sq);
+                        const float u = sc_odds(oa[e]), so = __builtin_amdgcn_rcpf(1.0f + u);
                         dh *= so;
-                        dov[e] = dh * h[i][e] * sq;
+                        dov[e] = dh * h[i][e] * (u * so);
                     }
-                    const float g = dh + carry[e], sv = s[i][e];
-                    const float a = sv < 0.5f ? 1.0f - sv : __builtin_amdgcn_exp2f(SC_LOG2E * fv[e]) * sv;
+                    const float g = dh + carry[e], sv = __builtin_amdgcn_rcpf(1.0f + odds[i][e]);
                     dx[e] = sv * g;
-                    df[e] = a * dx[e] * (hp - xv[e]);
+                    df[e] = -(odds[i][e] * sv * dx[e]) * xd[e];
                     cn[e] = __builtin_fmaf(-sv, g, g);
                 }
                 if (ok) carry = cn;                                 // uniform
                 else dx = df = dov = f32x2{0.f, 0.f};
-                if (decltype(full)::value || t < p.T) {
-                    Pair<KIND>::store(gx + t * dzst, dx);
-                    Pair<KIND>::store(gf + t * dzst, df);
-                    if constexpr (GATED) Pair<KIND>::store(go + t * dzst, dov);
+                if (FULL || t < p.T) {
+                    Pair<KIND>::store(gr + vg[0], dx);
+                    Pair<KIND>::store(gr + vg[1], df);
+                    if constexpr (GATED) Pair<KIND>::store(gr + vg[PARTS - 1], dov);
                 }
+                gr += p.reverse ? dzst : -dzst;
             });
         };
-        if ((kb + 1) * SC_STEPS <= w.len) block(std::integral_constant<bool, true>{});
-        else block(std::integral_constant<bool, false>{});
+        if (full_block) states(std::integral_constant<bool, true>{});
+        else states(std::integral_constant<bool, false>{});
+        __builtin_amdgcn_sched_barrier(0);
+        in.forget();
+        if (it + 1 < n) issue(p.reverse ? kb + 1 : kb - 1);
+        if (full_block) grads(std::integral_constant<bool, true>{});
+        else grads(std::integral_constant<bool, false>{});
     }
     if (p.dh0 != nullptr && w.ord == p.nchunk - 1) *(f32x2u*)(p.dh0 + (long long)w.b * p.D + w.cc) = carry;
 }
 
 // (M, v) of one chunk, backward: carry -> carry - M carry + v.
 template <int KIND, bool GATED, bool CODES>
-__global__ __launch_bounds__(256) void k_scan_bsum(ScanP p) {
+__global__ __launch_bounds__(64 * SC_GROUP) void k_scan_bsum(ScanP p) {
     typedef typename Pair<KIND>::raw raw;
     constexpr int PARTS = GATED ? 3 : 2, EB = Elem<KIND>::bytes;
-    const ScanAt w = scan_at(p, true);
-    if (!w.valid || w.ord == p.nchunk - 1) return;
+    const ScanAt w = scan_at<true>(p, true);
     const long long dyst = p.dy_st * EB;
-    const unsigned char* dyp = (const unsigned char*)p.dy + (w.b * p.dy_sb + w.cc) * EB;
-    const int vhi = (w.len + SC_STEPS - 1) / SC_STEPS, hi = w.hi < vhi ? w.hi : vhi, n = hi - w.lo;
+    const unsigned char* dyb = (const unsigned char*)p.dy + w.b * p.dy_sb * EB;
+    const unsigned dyoff[1] = {(unsigned)w.cc * EB};
+    const int vhi = (w.len + SC_STEPS - 1) / SC_STEPS, hi = w.hi < vhi ? w.hi : vhi;
+    const int n = w.ord < p.nchunk - 1 ? hi - w.lo : 0;
     f32x2 v{0.f, 0.f}, m{0.f, 0.f};
     ScanIn<KIND, PARTS, CODES> nin;
-    raw ndy[SC_STEPS];
+    raw ndy[1][SC_STEPS];
     auto issue = [&](int kb) {
-        nin.template load<1>(p, w, kb);
-        if constexpr (GATED) nin.template load<2>(p, w, kb);
-        if (p.dy != nullptr) sc_load_rows<KIND>(ndy, dyp, dyst, kb, p.T, p.reverse);
+        nin.template load<1, PARTS>(p, w, kb);
+        if (p.dy != nullptr) sc_load_rows<KIND, 0, 1>(ndy, dyb, dyst, dyoff, kb, p.T, p.reverse);
         else {
 #pragma unroll
-            for (int i = 0; i < SC_STEPS; ++i) ndy[i] = Pair<KIND>::zero();
+            for (int i = 0; i < SC_STEPS; ++i) ndy[0][i] = Pair<KIND>::zero();
         }
     };
     if (n > 0) issue(p.reverse ? w.lo : hi - 1);
@@ -482,27 +663,35 @@ __global__ __launch_bounds__(256) void k_scan_bsum(ScanP p) {
         const ScanIn<KIND, PARTS, CODES> in = nin;
         raw dy[SC_STEPS];
 #pragma unroll
-        for (int i = 0; i < SC_STEPS; ++i) dy[i] = ndy[i];
+        for (int i = 0; i < SC_STEPS; ++i) dy[i] = ndy[0][i];
+        const bool checked = in.lost();
         if (it + 1 < n) issue(p.reverse ? kb + 1 : kb - 1);
-        static_for<SC_STEPS>([&](auto jc) {
-            constexpr int i = SC_STEPS - 1 - decltype(jc)::value;
-            const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-            if (t < w.len) {                                        // uniform
-                const f32x2 fv = in.template get<1, i>(), dyv = Pair<KIND>::get(dy[i]);
+        auto block = [&](auto chk) {
+            constexpr bool CHECKED = decltype(chk)::value;
+            static_for<SC_STEPS>([&](auto jc) {
+                constexpr int i = SC_STEPS - 1 - decltype(jc)::value;
+                const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
+                if (t < w.len) {                                    // uniform
+                    const f32x2 fa = in.template times<1, i, CHECKED>(SC_LOG2E), dyv = Pair<KIND>::get(dy[i]);
+                    f32x2 oa;
+                    if constexpr (GATED) oa = in.template times<PARTS - 1, i, CHECKED>(-SC_LOG2E);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float dh = dyv[e];
-                    if constexpr (GATED) dh *= sigmoidf_(in.template get<2, i>()[e]);
-                    const float s = sc_share(fv[e]), g = dh + v[e];
-                    v[e] = __builtin_fmaf(-s, g, g);
-                    m[e] = __builtin_fmaf(s, 1.0f - m[e], m[e]);
+                    for (int e = 0; e < 2; ++e) {
+                        float dh = dyv[e];
+                        if constexpr (GATED) dh *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(oa[e]));
+                        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fa[e])), g = dh + v[e];
+                        v[e] = __builtin_fmaf(-s, g, g);
+                        m[e] = __builtin_fmaf(s, 1.0f - m[e], m[e]);
+                    }
                 }
-            }
-        });
+            });
+        };
+        if constexpr (CODES) {
+            if (checked) block(std::integral_constant<bool, true>{});
+            else block(std::integral_constant<bool, false>{});
+        } else block(std::integral_constant<bool, false>{});
     }
-    float* q = p.sums + ((long long)w.b * p.nchunk + w.ord) * 2 * p.D + w.cc;
-    *(f32x2u*)q = m;
-    *(f32x2u*)(q + p.D) = v;
+    scan_leave(p, w, m, v);
 }
 
 // One token.  `alive` (nullable): a sentence that has ended keeps its state and gives y = 0.  h_out may be h: every

@@ -25,11 +25,12 @@ constexpr int MAX_GRID = 0x7fffffff;
 bool known_kind(int kind) { return kind == SAD_SRC_F32 || kind == SAD_SRC_BF16 || kind == SAD_SRC_F16; }
 
 // ---- scan ---------------------------------------------------------------------------------------------------------
-// Time chunks of a sentence: one where the waves of all sentences and channel groups fill the card by themselves.
+// Time chunks of a sentence: one where the waves of all sentences and channel groups fill the card by themselves, or
+// where a sentence is so short that the second launch costs more than the cut saves.
 int scan_chunks(int B, int T, int D) {
     const long long waves = (long long)B * ceil_div(D, SC_CH);
     const int nblk = ceil_div(T, SC_STEPS);
-    if (waves >= 1024) return 1;
+    if (waves >= 1024 || nblk < 4) return 1;
     long long n = (2048 + waves - 1) / waves;
     if (n > 64) n = 64;
     if (n > nblk) n = nblk;
@@ -60,23 +61,29 @@ ScanP scan_params(const sad_scan_args* a, void* workspace) {
     p.h_last = a->h_last;
     p.kept = a->kept;
     p.codes = (unsigned char*)a->codes;
-    if (a->codes != nullptr)
-        p.exps = p.codes + (size_t)a->B * p.nblk * (a->gated ? 3 : 2) * a->D * SC_STEPS;
+    if (a->codes != nullptr) {
+        const size_t tiles = (size_t)a->B * p.nblk * (a->gated ? 3 : 2);
+        p.exps = p.codes + tiles * a->D * SC_STEPS;
+        p.lost = (unsigned*)(p.exps + tiles * ceil_div(a->D, C8_BLOCK) * SC_STEPS);
+    }
     p.dy = a->dy; p.dy_sb = a->dy_stride_b; p.dy_st = a->dy_stride_t;
     p.dh_last = a->dh_last;
     p.dz = a->dz; p.dz_sb = a->dz_stride_b; p.dz_st = a->dz_stride_t;
     p.dh0 = a->dh0;
     p.sums = (float*)workspace;
+    p.group = p.nchunk < SC_GROUP ? p.nchunk : SC_GROUP;
+    p.ngroup = ceil_div(p.nchunk, p.group);
     return p;
 }
 
 int scan_grid(const ScanP& p) { return (int)(((long long)p.B * p.ncg * p.nchunk + 3) / 4); }
+int scan_sum_grid(const ScanP& p) { return p.B * p.ncg * p.ngroup; }
 
 template <int KIND>
 int launch_scan_fwd(const sad_scan_args* a, const ScanP& p, hipStream_t st) {
     const dim3 grid(scan_grid(p)), block(256);
     if (p.nchunk > 1) {
-        hipLaunchKernelGGL((k_scan_sum<KIND>), grid, block, 0, st, p);
+        hipLaunchKernelGGL((k_scan_sum<KIND>), dim3(scan_sum_grid(p)), dim3(64 * p.group), 0, st, p);
         SAD_LAUNCHED("k_scan_sum");
     }
     const int save = p.codes != nullptr ? 2 : (p.kept != nullptr ? 1 : 0);
@@ -99,7 +106,7 @@ template <int KIND, bool GATED, bool CODES>
 int launch_scan_bwd(const ScanP& p, hipStream_t st) {
     const dim3 grid(scan_grid(p)), block(256);
     if (p.nchunk > 1) {
-        hipLaunchKernelGGL((k_scan_bsum<KIND, GATED, CODES>), grid, block, 0, st, p);
+        hipLaunchKernelGGL((k_scan_bsum<KIND, GATED, CODES>), dim3(scan_sum_grid(p)), dim3(64 * p.group), 0, st, p);
         SAD_LAUNCHED("k_scan_bsum");
     }
     hipLaunchKernelGGL((k_scan_bwd<KIND, GATED, CODES>), grid, block, 0, st, p);
@@ -153,7 +160,7 @@ extern "C" {
 size_t sad_gated_scan_workspace_bytes(int32_t B, int32_t T, int32_t D) {
     if (check_scan_dims(B, T, D, SAD_SRC_F32)) return 0;
     const int n = scan_chunks(B, T, D);
-    return n > 1 ? (size_t)B * n * 2 * D * sizeof(float) : 16;
+    return n > 1 ? (size_t)B * (n + ceil_div(n, n < SC_GROUP ? n : SC_GROUP)) * 2 * D * sizeof(float) : 16;
 }
 
 size_t sad_gated_scan_kept_bytes(int32_t B, int32_t T, int32_t D) {
@@ -163,7 +170,8 @@ size_t sad_gated_scan_kept_bytes(int32_t B, int32_t T, int32_t D) {
 
 size_t sad_gated_scan_codes_bytes(int32_t B, int32_t T, int32_t D, int32_t gated) {
     if (check_scan_dims(B, T, D, SAD_SRC_F32)) return 0;
-    return (size_t)B * ceil_div(T, SC_STEPS) * (gated ? 3 : 2) * ((size_t)D + ceil_div(D, C8_BLOCK)) * SC_STEPS;
+    const size_t blocks = (size_t)B * ceil_div(T, SC_STEPS);
+    return blocks * ((gated ? 3 : 2) * ((size_t)D + ceil_div(D, C8_BLOCK)) * SC_STEPS + ceil_div(D, SC_CH) * sizeof(unsigned));
 }
 
 int sad_gated_scan_fwd(const sad_scan_args* a, void* workspace, void* stream) {

@@ -678,18 +678,50 @@ def _need_device(t, what):
         raise RuntimeError("%s must be on the HIP device (got a CPU tensor); there is no CPU path" % what)
 
 
-def _bytes(nbytes, what, dev):
-    """Uninitialised device memory of a size the library names (0 = it refused)."""
-    if nbytes == 0:
-        raise RuntimeError("libsad %s failed: %s" % (what, _lib.last_error()))
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+# Sizes the library names, by (function, arguments): a call costs more host time than the lookup.
+_sizes = {}
+
+
+def _bytes(dev, name, *args):
+    """Uninitialised device memory of the size that the library's function `name` gives for `args` (0 = it refused)."""
+    n = _sizes.get((name, args))
+    if n is None:
+        n = getattr(_lib.load(), name)(*args)
+        if n == 0:
+            raise RuntimeError("libsad %s failed: %s" % (name, _lib.last_error()))
+        if len(_sizes) > 4096:
+            _sizes.clear()
+        _sizes[(name, args)] = n
+    return torch.empty(n, dtype=torch.uint8, device=dev)
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch(name, dev, *args):
+    """Library entry `name` with `args` and the current stream of `dev`."""
+    fn = getattr(_lib.load(), name)
+    cur = _current_device()
+    if dev.index is None or dev.index == cur:
+        rc = fn(*args, _RAW_STREAM(cur))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _RAW_STREAM(dev.index))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _like_rows(t, last):
     """New tensor [.., .., last] of t's type with the order of t's first two axes in memory."""
-    if t.stride(0) < t.stride(1) and t.shape[0] > 1 and t.shape[1] > 1:
-        return torch.empty((t.shape[1], t.shape[0], last), dtype=t.dtype, device=t.device).transpose(0, 1)
-    return torch.empty((t.shape[0], t.shape[1], last), dtype=t.dtype, device=t.device)
+    n0, n1, _ = t.shape
+    s0, s1, _ = t.stride()
+    if s0 < s1 and n0 > 1 and n1 > 1:
+        return torch.empty((n1, n0, last), dtype=t.dtype, device=t.device).transpose(0, 1)
+    return torch.empty((n0, n1, last), dtype=t.dtype, device=t.device)
 
 
 def _scan_parts(width, gated_output):
@@ -718,70 +750,60 @@ def _scan_lengths(lengths, B, T, dev):
     return lengths.to(device=dev, dtype=torch.int32, non_blocking=True).contiguous()
 
 
+def _scan_forward(z, h0, lengths, reverse, gated, int8, track):
+    B, T, W = z.shape
+    D = W // (3 if gated else 2)
+    dev = z.device
+    y = _like_rows(z, D)
+    h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
+    ws = _bytes(dev, "sad_gated_scan_workspace_bytes", B, T, D)
+    kept = _bytes(dev, "sad_gated_scan_kept_bytes", B, T, D) if track else None
+    codes = _bytes(dev, "sad_gated_scan_codes_bytes", B, T, D, int(gated)) if track and int8 else None
+    zs, ys = z.stride(), y.stride()
+    a = _lib.SadScanArgs(B, T, D, _KINDS[z.dtype], gated, reverse, z.data_ptr(), zs[0], zs[1], _addr(lengths), _addr(h0),
+                         y.data_ptr(), ys[0], ys[1], h_last.data_ptr(), _addr(kept), _addr(codes))
+    _launch("sad_gated_scan_fwd", dev, ctypes.byref(a), ws.data_ptr())
+    return y, h_last, kept, codes
+
+
 class _GatedScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, h0, lengths, reverse, gated, int8, track):
-        B, T = z.shape[:2]
-        D = z.shape[2] // (3 if gated else 2)
-        dev = z.device
-        lib = _lib.load()
-        y = _like_rows(z, D)
-        h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
-        kept = codes = None
-        ws = _bytes(lib.sad_gated_scan_workspace_bytes(B, T, D), "sad_gated_scan_workspace_bytes", dev)
-        if track:
-            kept = _bytes(lib.sad_gated_scan_kept_bytes(B, T, D), "sad_gated_scan_kept_bytes", dev)
-            if int8:
-                codes = _bytes(lib.sad_gated_scan_codes_bytes(B, T, D, gated), "sad_gated_scan_codes_bytes", dev)
-        a = _lib.SadScanArgs()
-        a.B, a.T, a.D, a.kind, a.gated, a.reverse = B, T, D, _KINDS[z.dtype], int(gated), int(reverse)
-        a.z, a.z_stride_b, a.z_stride_t = z.data_ptr(), z.stride(0), z.stride(1)
-        a.lengths = lengths.data_ptr() if lengths is not None else None
-        a.h0 = h0.data_ptr() if h0 is not None else None
-        a.y, a.y_stride_b, a.y_stride_t = y.data_ptr(), y.stride(0), y.stride(1)
-        a.h_last = h_last.data_ptr()
-        a.kept = kept.data_ptr() if kept is not None else None
-        a.codes = codes.data_ptr() if codes is not None else None
-        with _on(dev):
-            _lib.check(lib.sad_gated_scan_fwd(ctypes.byref(a), _ptr(ws), _stream_ptr()), "sad_gated_scan_fwd")
+    def forward(ctx, z, h0, lengths, reverse, gated, int8):
+        y, h_last, kept, codes = _scan_forward(z, h0, lengths, reverse, gated, int8, True)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(None if int8 else z, lengths, kept, codes)
-        ctx.scan = (B, T, D, z.dtype, tuple(z.shape), tuple(z.stride()), dev, reverse, gated)
+        ctx.scan = (z.dtype, z.shape, z.stride(), y.shape, reverse, gated, z.is_contiguous())
         return y, h_last
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh_last):
         z, lengths, kept, codes = ctx.saved_tensors
-        B, T, D, dtype, zshape, zstride, dev, reverse, gated = ctx.scan
+        dtype, zshape, zstride, yshape, reverse, gated, plain = ctx.scan
         if dy is None and dh_last is None:
-            return (None,) * 7
-        if dy is not None and dy.stride(2) != 1:
-            dy = dy.contiguous()
+            return (None,) * 6
+        B, T, D = yshape
+        dev = kept.device
+        if dy is not None:
+            if dy.stride(2) != 1:
+                dy = dy.contiguous()
+            ds = dy.stride()
+        else:
+            ds = (0, 0)
         if dh_last is not None:
             dh_last = dh_last.contiguous()
-        if _is_dense(zshape, zstride):
+        if not plain and _is_dense(zshape, zstride):
             dz = torch.empty_strided(zshape, zstride, dtype=dtype, device=dev)
         else:
             dz = torch.empty(zshape, dtype=dtype, device=dev)
+        gs = dz.stride()
         dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
-        lib = _lib.load()
-        ws = _bytes(lib.sad_gated_scan_workspace_bytes(B, T, D), "sad_gated_scan_workspace_bytes", dev)
-        a = _lib.SadScanArgs()
-        a.B, a.T, a.D, a.kind, a.gated, a.reverse = B, T, D, _KINDS[dtype], int(gated), int(reverse)
-        if z is not None:
-            a.z, a.z_stride_b, a.z_stride_t = z.data_ptr(), z.stride(0), z.stride(1)
-        a.lengths = lengths.data_ptr() if lengths is not None else None
-        a.kept = kept.data_ptr()
-        a.codes = codes.data_ptr() if codes is not None else None
-        if dy is not None:
-            a.dy, a.dy_stride_b, a.dy_stride_t = dy.data_ptr(), dy.stride(0), dy.stride(1)
-        a.dh_last = dh_last.data_ptr() if dh_last is not None else None
-        a.dz, a.dz_stride_b, a.dz_stride_t = dz.data_ptr(), dz.stride(0), dz.stride(1)
-        a.dh0 = dh0.data_ptr() if dh0 is not None else None
-        with _on(dev):
-            _lib.check(lib.sad_gated_scan_bwd(ctypes.byref(a), _ptr(ws), _stream_ptr()), "sad_gated_scan_bwd")
-        return (dz if ctx.needs_input_grad[0] else None, dh0) + (None,) * 5
+        ws = _bytes(dev, "sad_gated_scan_workspace_bytes", B, T, D)
+        a = _lib.SadScanArgs(B, T, D, _KINDS[dtype], gated, reverse, _addr(z), zstride[0], zstride[1], _addr(lengths), None,
+                             None, 0, 0, None, kept.data_ptr(), _addr(codes),
+                             _addr(dy), ds[0], ds[1], _addr(dh_last), dz.data_ptr(), gs[0], gs[1], _addr(dh0))
+        _launch("sad_gated_scan_bwd", dev, ctypes.byref(a), ws.data_ptr())
+        return (dz if ctx.needs_input_grad[0] else None, dh0, None, None, None, None)
 
 
 def gated_scan(z, h0=None, lengths=None, reverse=False, gated_output=True, save="input"):
@@ -818,17 +840,23 @@ def gated_scan(z, h0=None, lengths=None, reverse=False, gated_output=True, save=
         return y, (h0.clone() if h0 is not None else torch.zeros((B, D), dtype=torch.float32, device=z.device))
     if z.stride(2) != 1:
         z = z.contiguous()
-    track = torch.is_grad_enabled() and (z.requires_grad or (h0 is not None and h0.requires_grad))
-    return _GatedScan.apply(z, h0.contiguous() if h0 is not None else None, lengths, bool(reverse), bool(gated_output),
-                            save == "int8", track)
+    if h0 is not None:
+        h0 = h0.contiguous()
+    if torch.is_grad_enabled() and (z.requires_grad or (h0 is not None and h0.requires_grad)):
+        return _GatedScan.apply(z, h0, lengths, bool(reverse), bool(gated_output), save == "int8")
+    return _scan_forward(z, h0, lengths, bool(reverse), bool(gated_output), False, False)[:2]
 
 
 def _overlaps(a, b):
-    """Do the address ranges of two tensors meet?"""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    """Do the address ranges of two non-empty matrices meet?"""
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    return a.data_ptr() + ((a.shape[0] - 1) * a.stride(0) + (a.shape[1] - 1) * a.stride(1) + 1) * a.element_size() > b.data_ptr()
+
+
+def _need_state(h, name, B, D, dev):
+    if h.dtype != torch.float32 or tuple(h.shape) != (B, D) or h.device != dev or h.stride(1) != 1:
+        raise RuntimeError("%s must be float32 [%d,%d] with unit channel stride on %s" % (name, B, D, dev))
 
 
 def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
@@ -844,19 +872,20 @@ def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
     B, dev = z.shape[0], z.device
     if torch.is_grad_enabled() and (z.requires_grad or h.requires_grad):
         raise RuntimeError("gated_scan_step has no gradient: call it under torch.no_grad(), or train with gated_scan")
-    for t, name in ((h, "h"), (h_out, "h_out")):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, D) or t.device != dev or t.stride(1) != 1):
-            raise RuntimeError("%s must be float32 [%d,%d] with unit channel stride on %s" % (name, B, D, dev))
+    _need_state(h, "h", B, D, dev)
     if alive is not None and (alive.dtype not in (torch.bool, torch.uint8) or tuple(alive.shape) != (B,) or alive.device != dev):
         raise RuntimeError("alive must be a bool [%d] tensor on %s" % (B, dev))
     if h_out is None:
         h_out = torch.empty((B, D), dtype=torch.float32, device=dev)
-    elif B and (B > 1 and h_out.stride(0) < D):
-        raise RuntimeError("rows of h_out overlap")
-    elif B and (h_out.data_ptr(), h_out.stride()) != (h.data_ptr(), h.stride()) and _overlaps(h_out, h):
-        raise RuntimeError("h_out must be h itself or must not overlap it")
-    if B and _overlaps(h_out, z):
-        raise RuntimeError("h_out must not overlap z")
+    else:
+        if h_out is not h:
+            _need_state(h_out, "h_out", B, D, dev)
+            if B and (h_out.data_ptr() != h.data_ptr() or h_out.stride() != h.stride()) and _overlaps(h_out, h):
+                raise RuntimeError("h_out must be h itself or must not overlap it")
+        if B > 1 and h_out.stride(0) < D:
+            raise RuntimeError("rows of h_out overlap")
+        if B and _overlaps(h_out, z):
+            raise RuntimeError("h_out must not overlap z")
     _need_device(z, "z")
     y = torch.empty((B, D), dtype=z.dtype, device=dev)
     if B == 0:
@@ -865,10 +894,8 @@ def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
         z = z.contiguous()
     if alive is not None:
         alive = alive.contiguous()
-    with _on(dev):
-        _lib.check(_lib.load().sad_gated_scan_step(B, D, kind, int(gated_output), _ptr(z), z.stride(0), _ptr(h), h.stride(0), _ptr(alive),
-                                                   _ptr(y), y.stride(0), _ptr(h_out), h_out.stride(0), _stream_ptr()),
-                   "sad_gated_scan_step")
+    _launch("sad_gated_scan_step", dev, B, D, kind, int(gated_output), z.data_ptr(), z.stride(0), h.data_ptr(), h.stride(0), _addr(alive),
+            y.data_ptr(), D, h_out.data_ptr(), h_out.stride(0))
     return y, h_out
 
 
@@ -899,9 +926,8 @@ class Checkpoint8:
         out = torch.empty(self.shape, dtype=self.dtype, device=self.saved.device)
         if out.numel():
             C = self.shape[-1]
-            with _on(out.device):
-                _lib.check(_lib.load().sad_checkpoint8_restore(out.numel() // C, C, _KINDS[self.dtype], _ptr(self.saved), _ptr(out),
-                                                               _stream_ptr()), "sad_checkpoint8_restore")
+            _launch("sad_checkpoint8_restore", out.device, out.numel() // C, C, _KINDS[self.dtype], self.saved.data_ptr(),
+                    out.data_ptr())
         return out
 
 
@@ -920,10 +946,8 @@ def checkpoint8(x):
         return Checkpoint8(torch.empty(0, dtype=torch.uint8, device=dev), shape, x.dtype)
     x, n0, n1, s0, s1 = _rows2(x)
     C = shape[-1]
-    lib = _lib.load()
-    saved = _bytes(lib.sad_checkpoint8_bytes(n0 * n1, C), "sad_checkpoint8_bytes", dev)
-    with _on(dev):
-        _lib.check(lib.sad_checkpoint8_save(n0, n1, C, kind, _ptr(x), s0, s1, _ptr(saved), _stream_ptr()), "sad_checkpoint8_save")
+    saved = _bytes(dev, "sad_checkpoint8_bytes", n0 * n1, C)
+    _launch("sad_checkpoint8_save", dev, n0, n1, C, kind, x.data_ptr(), s0, s1, saved.data_ptr())
     return Checkpoint8(saved, shape, x.dtype)
 
 
@@ -947,13 +971,11 @@ def weight_grad8(dy, ckpt, bias=False):
             return dw
         return dw, (torch.zeros(N, dtype=torch.float32, device=dev) if dy.numel() == 0 else dy.float().flatten(0, -2).sum(0))
     dy, n0, n1, s0, s1 = _rows2(dy)
-    lib = _lib.load()
     dw = torch.empty((N, K), dtype=torch.float32, device=dev)
     db = torch.empty(N, dtype=torch.float32, device=dev) if bias else None
-    ws = _bytes(lib.sad_weight_grad8_workspace_bytes(n0 * n1, N, K), "sad_weight_grad8_workspace_bytes", dev)
-    with _on(dev):
-        _lib.check(lib.sad_weight_grad8(n0, n1, N, K, kind, _ptr(dy), s0, s1, _ptr(ckpt.saved), _ptr(dw), _ptr(db), _ptr(ws),
-                                        _stream_ptr()), "sad_weight_grad8")
+    ws = _bytes(dev, "sad_weight_grad8_workspace_bytes", n0 * n1, N, K)
+    _launch("sad_weight_grad8", dev, n0, n1, N, K, kind, dy.data_ptr(), s0, s1, ckpt.saved.data_ptr(), dw.data_ptr(), _addr(db),
+            ws.data_ptr())
     return (dw, db) if bias else dw
 
 
