@@ -402,7 +402,7 @@ int sad_checkpoint8_save(int64_t n0, int64_t n1, int64_t C, int32_t kind, const 
 int sad_checkpoint8_restore(int64_t rows, int64_t C, int32_t kind, const void* saved, void* out, void* stream);
 /* dw [N,K] = dy^T x^ (and db [N] = column sums of dy, or NULL) with dy [n0,n1,N] and x^ the values of a checkpoint of
  * n0 * n1 rows of K channels; fp32 sums, the same result at every call. */
-size_t sad_weight_grad8_workspace_bytes(int64_t rows, int64_t N, int64_t K);
+size_t sad_weight_grad8_workspace_bytes(int64_t rows, int64_t N, int64_t K, int32_t kind);
 int sad_weight_grad8(int64_t n0, int64_t n1, int64_t N, int64_t K, int32_t kind, const void* dy, int64_t stride0, int64_t stride1,
                      const void* saved, float* dw, float* db, void* workspace, void* stream);
 

@@ -6,6 +6,8 @@
 #include "ckpt8.hpp"
 #include "wgrad8.hpp"
 
+#include <mutex>
+
 using namespace sad;
 
 namespace {
@@ -23,6 +25,21 @@ namespace {
 constexpr int MAX_GRID = 0x7fffffff;
 
 bool known_kind(int kind) { return kind == SAD_SRC_F32 || kind == SAD_SRC_BF16 || kind == SAD_SRC_F16; }
+
+// More than 64 KB of dynamic LDS have to be allowed once per kernel and device.
+hipError_t allow_dynamic_lds(const void* kernel, int bytes) {
+    static std::mutex mu;
+    static const void* done[64][16];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+    std::lock_guard<std::mutex> lock(mu);
+    int i = 0;
+    for (; i < 16 && done[dev][i] != nullptr; ++i)
+        if (done[dev][i] == kernel) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess && i < 16) done[dev][i] = kernel;
+    return e;
+}
 
 // ---- scan ---------------------------------------------------------------------------------------------------------
 // Time chunks of a sentence: one where the waves of all sentences and channel groups fill the card by themselves, or
@@ -136,21 +153,53 @@ int check_matrix(int64_t rows, int64_t C, int kind) {
 }
 
 // ---- weight gradient --------------------------------------------------------------------------------------------------
-struct Split { int tn, tk, splits, rows; };
-// Row splits: enough workgroups for two rounds of the card's 256 CUs, no split shorter than 512 rows.
-Split wgrad8_split(int64_t M, int64_t N, int64_t K) {
-    Split s;
-    s.tn = (int)((N + W8_BN - 1) / W8_BN);
-    s.tk = (int)((K + W8_BK - 1) / W8_BK);
-    const int64_t tiles = (int64_t)s.tn * s.tk;
-    int64_t n = (512 + tiles - 1) / tiles, most = (M + 511) / 512;
-    if (n > most) n = most;
-    if (n < 1) n = 1;
-    int64_t rows = (M + n - 1) / n;
-    rows = (rows + W8_BM - 1) / W8_BM * W8_BM;
-    s.rows = (int)rows;
-    s.splits = (int)((M + rows - 1) / rows);
-    return s;
+// Tile and row splits by an estimate of the time: rounds of workgroups over the 256 CUs, each round as long as its rows
+// take at the tile's rate, and the slab of the splits once written and once read.  Rates measured on [16384, 6144, 2048]
+// and [32768, 1536, 300]: see k_wgrad8.
+struct Split { int bn, bk, tn, tk, splits, rows; };
+Split wgrad8_split(int64_t M, int64_t N, int64_t K, int kind) {
+    struct Tile { int bn, bk; double us_per_row; };        // time of one workgroup per token row
+    static const Tile wide[] = {{256, 256, 0.0140}, {192, 256, 0.0115}, {128, 128, 0.0065}};
+    static const Tile fp32[] = {{128, 128, 0.0180}};
+    const Tile* t = kind == SAD_SRC_F32 ? fp32 : wide;
+    const int nt = kind == SAD_SRC_F32 ? 1 : 3;
+    Split best{};
+    double best_us = 1e30;
+    for (int i = 0; i < nt; ++i) {
+        const int64_t tn = (N + t[i].bn - 1) / t[i].bn, tk = (K + t[i].bk - 1) / t[i].bk;
+        for (int64_t n = 1; n <= 64; ++n) {
+            int64_t rows = (M + n - 1) / n;
+            rows = (rows + 63) / 64 * 64;
+            const int64_t splits = (M + rows - 1) / rows;
+            if (splits != n && n > 1) continue;
+            if (n > 1 && rows < 256) break;
+            const int64_t rounds = (tn * tk * splits + 255) / 256;
+            const double us = 3.0 + rounds * (rows * t[i].us_per_row + 2.0) + (splits > 1 ? 3.0 + (splits + 1.0) * 2 * 4 * N * K / 4.0e6 : 0.0);
+            if (us < best_us) {
+                best_us = us;
+                best = Split{t[i].bn, t[i].bk, (int)tn, (int)tk, (int)splits, (int)rows};
+            }
+        }
+    }
+    return best;
+}
+
+template <int KIND, int BN, int BK, int W1, int W2>
+int launch_wgrad8(const Wgrad8P& p, hipStream_t st) {
+    typedef W8<KIND, BN, BK, W1, W2> W;
+    if (allow_dynamic_lds((const void*)k_wgrad8<W>, W::LDS) != hipSuccess) return set_error(-2, "k_wgrad8: %d bytes of LDS refused", W::LDS);
+    hipLaunchKernelGGL((k_wgrad8<W>), dim3(8u * p.per_xcd), dim3(W::NT), W::LDS, st, p);
+    SAD_LAUNCHED("k_wgrad8");
+    return 0;
+}
+
+template <int KIND>
+int launch_wgrad8(const Wgrad8P& p, const Split& s, hipStream_t st) {
+    if constexpr (KIND != SAD_SRC_F32) {
+        if (s.bn == 256) return launch_wgrad8<KIND, 256, 256, 2, 4>(p, st);
+        if (s.bn == 192) return launch_wgrad8<KIND, 192, 256, 2, 4>(p, st);
+    }
+    return launch_wgrad8<KIND, 128, 128, 2, 2>(p, st);
 }
 
 }  // namespace
@@ -260,9 +309,9 @@ int sad_checkpoint8_restore(int64_t rows, int64_t C, int32_t kind, const void* s
     return 0;
 }
 
-size_t sad_weight_grad8_workspace_bytes(int64_t rows, int64_t N, int64_t K) {
-    if (check_matrix(rows, K, SAD_SRC_F32) || check_matrix(rows, N, SAD_SRC_F32)) return 0;
-    const Split s = wgrad8_split(rows, N, K);
+size_t sad_weight_grad8_workspace_bytes(int64_t rows, int64_t N, int64_t K, int32_t kind) {
+    if (check_matrix(rows, K, kind) || check_matrix(rows, N, kind)) return 0;
+    const Split s = wgrad8_split(rows, N, K, kind);
     return s.splits > 1 ? (size_t)s.splits * (N * K + N) * sizeof(float) : 16;
 }
 
@@ -277,7 +326,7 @@ int sad_weight_grad8(int64_t n0, int64_t n1, int64_t N, int64_t K, int32_t kind,
     SAD_NEED(dw, "dw");
     SAD_NEED(workspace, "workspace");
     if ((size_t)saved % 16) return set_error(-1, "saved must be 16-byte aligned");
-    const Split s = wgrad8_split(M, N, K);
+    const Split s = wgrad8_split(M, N, K, kind);
     const int64_t groups = (int64_t)s.tn * s.tk * s.splits;
     if (groups > MAX_GRID) return set_error(-1, "N=%lld x K=%lld beyond the supported maximum", (long long)N, (long long)K);
     Wgrad8P p{};
@@ -286,15 +335,21 @@ int sad_weight_grad8(int64_t n0, int64_t n1, int64_t N, int64_t K, int32_t kind,
     p.dy = dy;
     p.yr = Rows2{stride0, stride1, (unsigned)n1};
     p.y_flat = n0 == 1 || stride0 == n1 * stride1;
+    // Chunks of 8 columns reach `over` entries past a row's end where N is no multiple of 8: memory of the rows behind, which
+    // is there for all rows but the last few.
+    const int64_t over = (8 - N % 8) % 8;
+    p.fast_rows = !p.y_flat ? 0 : (over == 0 ? (int)M : (stride1 > 0 ? (int)(M - (over + stride1 - 1) / stride1) : 0));
     p.codes = (const unsigned char*)saved;
     p.exps = p.codes + (size_t)M * p.Kp;
+    p.per_xcd = (int)((groups + 7) / 8);
     p.tn = s.tn; p.tk = s.tk; p.splits = s.splits; p.rows = s.rows;
     float* part_b = (float*)workspace + (size_t)s.splits * N * K;
     p.out = s.splits > 1 ? (float*)workspace : dw;
     p.out_b = db == nullptr ? nullptr : (s.splits > 1 ? part_b : db);
     hipStream_t st = (hipStream_t)stream;
-    BY_KIND(kind, hipLaunchKernelGGL((k_wgrad8<KIND>), dim3((unsigned)groups), dim3(256), W8<KIND>::LDS, st, p));
-    SAD_LAUNCHED("k_wgrad8");
+    int rc = 0;
+    BY_KIND(kind, rc = launch_wgrad8<KIND>(p, s, st));
+    if (rc != 0) return rc;
     if (s.splits > 1) {
         const long long n = (long long)N * K;
         long long g = (n + 255) / 256;

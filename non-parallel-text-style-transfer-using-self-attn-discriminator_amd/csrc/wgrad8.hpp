@@ -4,200 +4,280 @@
 //
 // X^ is decoded on its way into LDS; its values are exact in bf16 and fp16 (ckpt8.hpp), so the products are those of dY
 // with the checkpoint and nothing is rounded but the fp32 sums.  dY in float32 is split into three bf16 parts
-// (8 + 8 + 8 significant bits, exact), one matrix instruction each.
+// (8 + 8 + 8 significant bits, exact), one matrix instruction each.  db is one more column of ones for the matrix
+// instructions of the workgroups of the first k tile.
 //
 // Both operands are stored with the reduced index slow, so fragments are read from LDS with the transposing read
-// (tr_frag).  Token rows are split over workgroups where the output has few tiles; the partial tiles go to a
-// slab and a second launch adds them in fixed order (no atomics: the result does not depend on scheduling).
+// (tr_frag).  Token rows are split over workgroups where the output has few tiles; the partial tiles go to a slab and a
+// second launch adds them in fixed order (no atomics: the result does not depend on scheduling).
+//
+// Pipeline, one barrier per stage of 64 rows: stage s is multiplied out of one LDS buffer while stage s + 1 moves from
+// registers (decoded) into the other and the loads of stage s + 2 are issued.  Half of the waves stage first and multiply
+// then, the other half the other way round, and each SIMD holds one of each: the decoding (vector) of one overlaps the
+// matrix instructions of the other.
 #pragma once
 #include "ckpt8.hpp"
 #include "gemm_core.hpp"
 
 namespace sad {
 
-constexpr int W8_BN = 128, W8_BK = 128, W8_BM = 64;        // outputs n, outputs k, token rows per stage
-constexpr int W8_PITCH = W8_BN * 2 + 32;                   // LDS row pitch in bytes: odd multiple of 32 (tr_frag)
-template <int KIND> struct W8 {
-    static constexpr int PLANES = KIND == SAD_SRC_F32 ? 3 : 1;              // bf16 / fp16 images of dY
-    static constexpr int LDS = W8_BM * W8_PITCH * (PLANES + 1);
+// Workgroup tile BN x BK outputs, W1 x W2 waves.
+template <int KIND_, int BN_, int BK_, int W1_, int W2_> struct W8 {
+    static constexpr int KIND = KIND_, BN = BN_, BK = BK_, W1 = W1_, W2 = W2_;
+    static constexpr int BM = 64;                              // token rows per stage
+    static constexpr int NT = 64 * W1 * W2;
+    static constexpr int T1 = BN / W1 / 16, T2 = BK / W2 / 16;
+    static constexpr int PLANES = KIND == SAD_SRC_F32 ? 3 : 1; // bf16 / fp16 images of dY
+    static constexpr int PA = BN * 2 + 32, PB = BK * 2 + 32;   // LDS row pitch in bytes: odd multiples of 32 (tr_frag)
+    static constexpr int ABYTES = BM * PA, BUF = PLANES * ABYTES + BM * PB;
+    static constexpr int LDS = 2 * BUF;
+    static constexpr int CA = BN / 8, CB = BK / 16;            // chunks of a row: 8 entries of dY, 16 codes
+    static constexpr int NA = BM * CA / NT, NB = BM * CB / NT; // chunks per thread
+    static_assert(BM * CA % NT == 0 && BM * CB % NT == 0, "staging must divide evenly");
+    static_assert(BN % (W1 * 16) == 0 && BK % (W2 * 16) == 0 && (BN / 16) % 2 == 0 && (BK / 16) % 2 == 0, "tile");
 };
 
 struct Wgrad8P {
     int M, N, K, Kp;              // Kp: K rounded up to 32 (pitch of the codes)
     const void* dy; Rows2 yr; int y_flat;      // y_flat: row m starts at m * yr.s1
+    int fast_rows;                // rows in front of this one may be read in whole chunks of 8 columns
     const unsigned char* codes; const unsigned char* exps;
     float* out;                   // [splits][N][K], or dW itself when splits == 1
     float* out_b;                 // [splits][N] or db; NULL: no bias
-    int tn, tk, splits, rows;     // tiles, row splits, rows per split (multiple of W8_BM)
+    int tn, tk, splits, rows;     // tiles, row splits, rows per split (multiple of 64)
+    int per_xcd;                  // workgroups per XCD
 };
 
-// 8 columns of dY from c on, as loaded
+// 8 entries of dY as loaded
 template <int KIND> struct DyChunk { u32x4 v; };
 template <> struct DyChunk<SAD_SRC_F32> { f32x4 a, b; };
 
-template <int KIND>
-__global__ __launch_bounds__(256) void k_wgrad8(Wgrad8P p) {
-    constexpr int PLANES = W8<KIND>::PLANES, PLANE = W8_BM * W8_PITCH, CH = W8_BM * (W8_BN / 8) / 256;
-    extern __shared__ __align__(16) unsigned char lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, w1 = wave >> 1, w2 = wave & 1;
-    const int tile = blockIdx.x % (p.tn * p.tk), split = blockIdx.x / (p.tn * p.tk);
-    const int n0 = (tile / p.tk) * W8_BN, k0 = (tile % p.tk) * W8_BK;
-    const int m_begin = split * p.rows, m_end = m_begin + p.rows < p.M ? m_begin + p.rows : p.M;
-    const int cc = tid & 15, rr = tid >> 4;                  // this thread's 8-column chunk and first row of a stage
-    const int cn = n0 + cc * 8, ck = k0 + cc * 8;
-    const int nfull = p.N - cn;                              // columns of dY left from cn on
-    const bool kin = ck < p.Kp;
-    DyChunk<KIND> ra[CH];
-    u32x2 rb[CH];
-    unsigned re[CH];
-    f32x4 acc[4][4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float bias[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ unsigned c8_pack16(float a, float b, bool half) {
+    if (half) return (unsigned)__builtin_bit_cast(unsigned short, (_Float16)a) | ((unsigned)__builtin_bit_cast(unsigned short, (_Float16)b) << 16);
+    // exact in bf16: the upper halves
+    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
+}
 
-    auto issue = [&](int m0) {
+template <class W>
+__global__ __launch_bounds__(W::NT) void k_wgrad8(Wgrad8P p) {
+    constexpr int KIND = W::KIND, EB = Elem<KIND>::bytes;
+    extern __shared__ __align__(16) unsigned char lds[];
+    // Consecutive workgroups go to the 8 XCDs in turn.  Each XCD takes a compact block of tiles (4 k tiles wide), so that
+    // the rows its workgroups stream at the same time are shared in its L2.
+    const int unit = (int)(blockIdx.x & 7) * p.per_xcd + (int)(blockIdx.x >> 3);
+    const int tiles = p.tn * p.tk;
+    if (unit >= tiles * p.splits) return;
+    const int split = unit / tiles, o = unit - split * tiles;
+    const int kg = o / (4 * p.tn), gw = p.tk - kg * 4 < 4 ? p.tk - kg * 4 : 4, r = o - kg * 4 * p.tn;
+    const int n0 = (r / gw) * W::BN, k0 = (kg * 4 + r % gw) * W::BK;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w1 = wave / W::W2, w2 = wave % W::W2;
+    const int m_begin = split * p.rows, m_end = m_begin + p.rows < p.M ? m_begin + p.rows : p.M;
+    const int nst = (m_end - m_begin + W::BM - 1) / W::BM;
+    const bool bias = p.out_b != nullptr && k0 == 0;
+
+    // this thread's chunks of a stage
+    int arow[W::NA], acol[W::NA], brow[W::NB], bcol[W::NB];
+    const unsigned char* ap[W::NA];
+    const unsigned char* bp[W::NB];
+    const unsigned char* ep[W::NB];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int m = m0 + rr + 16 * i;
-            const bool ok = m < m_end;
-            if constexpr (KIND == SAD_SRC_F32) ra[i].a = ra[i].b = f32x4{0.f, 0.f, 0.f, 0.f};
-            else ra[i].v = u32x4{0u, 0u, 0u, 0u};
-            rb[i] = u32x2{0u, 0u};
-            re[i] = 1u;
-            if (ok && nfull > 0) {
-                const long long off = (p.y_flat ? (long long)m * p.yr.s1 : p.yr.at((unsigned)m)) + cn;
+    for (int i = 0; i < W::NA; ++i) {
+        const int g = tid + i * W::NT;
+        arow[i] = g / W::CA;
+        acol[i] = (g - arow[i] * W::CA) * 8;
+        // chunks that lie past the last column read the first one (their products are not stored)
+        ap[i] = (const unsigned char*)p.dy + ((long long)(m_begin + arow[i]) * p.yr.s1 + (n0 + acol[i] < p.N ? n0 + acol[i] : 0)) * EB;
+    }
+#pragma unroll
+    for (int i = 0; i < W::NB; ++i) {
+        const int g = tid + i * W::NT;
+        brow[i] = g / W::CB;
+        bcol[i] = (g - brow[i] * W::CB) * 16;
+        const int c = k0 + bcol[i] < p.Kp ? k0 + bcol[i] : 0;
+        bp[i] = p.codes + (long long)(m_begin + brow[i]) * p.Kp + c;
+        ep[i] = p.exps + (long long)(m_begin + brow[i]) * (p.Kp / C8_BLOCK) + c / C8_BLOCK;
+    }
+    const long long astep = (long long)W::BM * p.yr.s1 * EB, bstep = (long long)W::BM * p.Kp, estep = bstep / C8_BLOCK;
+
+    DyChunk<KIND> ra[W::NA];
+    u32x4 rb[W::NB];
+    unsigned re[W::NB];
+    auto issue = [&](int s) {
+        const int m0 = m_begin + s * W::BM;
+        if (m0 + W::BM <= p.fast_rows && m0 + W::BM <= m_end) {
+#pragma unroll
+            for (int i = 0; i < W::NA; ++i) {
                 if constexpr (KIND == SAD_SRC_F32) {
-                    const float* q = (const float*)p.dy + off;
-                    if (nfull >= 8) { ra[i].a = *(const f32x4u*)q; ra[i].b = *(const f32x4u*)(q + 4); }
+                    ra[i].a = *(const f32x4u*)ap[i];
+                    ra[i].b = *(const f32x4u*)(ap[i] + 16);
+                } else ra[i].v = *(const u32x4h*)ap[i];
+            }
+#pragma unroll
+            for (int i = 0; i < W::NB; ++i) {
+                rb[i] = *(const u32x4*)bp[i];
+                re[i] = *ep[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W::NA; ++i) {
+                if constexpr (KIND == SAD_SRC_F32) ra[i].a = ra[i].b = f32x4{0.f, 0.f, 0.f, 0.f};
+                else ra[i].v = u32x4{0u, 0u, 0u, 0u};
+                const int m = m0 + arow[i], c = n0 + acol[i];
+                if (m < m_end) {
+                    const long long off = (p.y_flat ? (long long)m * p.yr.s1 : p.yr.at((unsigned)m)) + c;
+                    if constexpr (KIND == SAD_SRC_F32) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (c + j < p.N) ra[i].a[j] = ((const float*)p.dy)[off + j];
+                            if (c + 4 + j < p.N) ra[i].b[j] = ((const float*)p.dy)[off + 4 + j];
+                        }
+                    } else if (c + 8 <= p.N) ra[i].v = *(const u32x4h*)((const unsigned short*)p.dy + off);
                     else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float v = j < nfull ? q[j] : 0.f;
-                            if (j < 4) ra[i].a[j] = v; else ra[i].b[j - 4] = v;
-                        }
-                    }
-                } else {
-                    const unsigned short* q = (const unsigned short*)p.dy + off;
-                    if (nfull >= 8) ra[i].v = *(const u32x4h*)q;
-                    else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const unsigned v = j < nfull ? q[j] : 0u;
-                            ra[i].v[j >> 1] |= v << (16 * (j & 1));
-                        }
+                        for (int j = 0; j < 8; ++j)
+                            if (c + j < p.N) ra[i].v[j >> 1] |= (unsigned)((const unsigned short*)p.dy)[off + j] << (16 * (j & 1));
                     }
                 }
             }
-            if (ok && kin) {
-                rb[i] = *(const u32x2*)(p.codes + (long long)m * p.Kp + ck);
-                re[i] = p.exps[(long long)m * (p.Kp / C8_BLOCK) + ck / C8_BLOCK];
+#pragma unroll
+            for (int i = 0; i < W::NB; ++i) {
+                rb[i] = u32x4{0u, 0u, 0u, 0u};
+                re[i] = 1u;
+                if (m0 + brow[i] < m_end) {
+                    rb[i] = *(const u32x4*)bp[i];
+                    re[i] = *ep[i];
+                }
             }
         }
+#pragma unroll
+        for (int i = 0; i < W::NA; ++i) ap[i] += astep;
+#pragma unroll
+        for (int i = 0; i < W::NB; ++i) { bp[i] += bstep; ep[i] += estep; }
     };
-    auto stage = [&]() {
+    auto stage = [&](unsigned char* buf) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            unsigned char* at = lds + (rr + 16 * i) * W8_PITCH + cc * 16;
-            float v[8];
+        for (int i = 0; i < W::NA; ++i) {
+            unsigned char* at = buf + arow[i] * W::PA + acol[i] * 2;
             if constexpr (KIND == SAD_SRC_F32) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = j < 4 ? ra[i].a[j] : ra[i].b[j - 4];
                 float rest[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) rest[j] = v[j];
+                for (int j = 0; j < 8; ++j) rest[j] = j < 4 ? ra[i].a[j] : ra[i].b[j - 4];
 #pragma unroll
                 for (int q = 0; q < 3; ++q) {
-                    u32x4 o;
+                    u32x4 v;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        o[j] = pack_bf16x2(rest[2 * j], rest[2 * j + 1]);
-                        rest[2 * j] -= __builtin_bit_cast(float, o[j] << 16);
-                        rest[2 * j + 1] -= __builtin_bit_cast(float, o[j] & 0xffff0000u);
+                        v[j] = pack_bf16x2(rest[2 * j], rest[2 * j + 1]);
+                        rest[2 * j] -= __builtin_bit_cast(float, v[j] << 16);
+                        rest[2 * j + 1] -= __builtin_bit_cast(float, v[j] & 0xffff0000u);
                     }
-                    *(u32x4*)(at + q * PLANE) = o;
+                    *(u32x4*)(at + q * W::ABYTES) = v;
                 }
-            } else {
-                *(u32x4*)at = ra[i].v;
+            } else *(u32x4*)at = ra[i].v;
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const unsigned short h = (unsigned short)(ra[i].v[j >> 1] >> (16 * (j & 1)));
-                    v[j] = KIND == SAD_SRC_BF16 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) bias[j] += v[j];
+        for (int i = 0; i < W::NB; ++i) {
             const float scale = c8_scale((int)re[i]);
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                x[4 * j + 0] = c8_value_checked<0>(rb[i][j], scale);
-                x[4 * j + 1] = c8_value_checked<1>(rb[i][j], scale);
-                x[4 * j + 2] = c8_value_checked<2>(rb[i][j], scale);
-                x[4 * j + 3] = c8_value_checked<3>(rb[i][j], scale);
-            }
-            u32x4 o;
+            u32x4 v[2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if constexpr (KIND == SAD_SRC_F16)
-                    o[j] = (unsigned)__builtin_bit_cast(unsigned short, (_Float16)x[2 * j]) |
-                           ((unsigned)__builtin_bit_cast(unsigned short, (_Float16)x[2 * j + 1]) << 16);
-                else o[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+                const unsigned w = rb[i][j];
+                v[j >> 1][(j & 1) * 2] = c8_pack16(c8_value<0>(w, scale), c8_value<1>(w, scale), KIND == SAD_SRC_F16);
+                v[j >> 1][(j & 1) * 2 + 1] = c8_pack16(c8_value<2>(w, scale), c8_value<3>(w, scale), KIND == SAD_SRC_F16);
             }
-            *(u32x4*)(at + PLANES * PLANE) = o;
+            const unsigned lost = c8_any_lost(rb[i][0]) | c8_any_lost(rb[i][1]) | c8_any_lost(rb[i][2]) | c8_any_lost(rb[i][3]);
+            if (__any(lost != 0u)) {      // a lost entry's NaN
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (((rb[i][j >> 2] >> (8 * (j & 3))) & 0xffu) == C8_LOST) v[j >> 3][(j >> 1) & 3] |= 0x7fffu << (16 * (j & 1));
+            }
+            unsigned char* at = buf + W::PLANES * W::ABYTES + brow[i] * W::PB + bcol[i] * 2;
+            *(u32x4*)at = v[0];
+            *(u32x4*)(at + 16) = v[1];
         }
     };
+
+    f32x4 acc[W::T1][W::T2], accb[2];
+#pragma unroll
+    for (int a = 0; a < W::T1; ++a)
+#pragma unroll
+        for (int b = 0; b < W::T2; ++b) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    accb[0] = accb[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const unsigned one = KIND == SAD_SRC_F16 ? 0x3c003c00u : 0x3f803f80u;
+    const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{one, one, one, one});
+    auto mma = [](bf16x8 a, bf16x8 b, f32x4 c) {
+        if constexpr (KIND == SAD_SRC_F16)
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    };
     const int rowsel = 4 * (lane >> 4) + ((lane >> 2) & 3), p4 = (lane & 3) * 4;
-    const unsigned char* abase = lds + rowsel * W8_PITCH + (w1 * 64 + p4) * 2;
-    const unsigned char* bbase = lds + PLANES * PLANE + rowsel * W8_PITCH + (w2 * 64 + p4) * 2;
-    issue(m_begin);
-    for (int m0 = m_begin; m0 < m_end; m0 += W8_BM) {
-        stage();
-        __syncthreads();
-        if (m0 + W8_BM < m_end) issue(m0 + W8_BM);
+    const int aoff = rowsel * W::PA + (w1 * (W::BN / W::W1) + p4) * 2;
+    const int boff = W::PLANES * W::ABYTES + rowsel * W::PB + (w2 * (W::BK / W::W2) + p4) * 2;
+    auto multiply = [&](const unsigned char* buf) {
 #pragma unroll
-        for (int ks = 0; ks < W8_BM / 32; ++ks) {
-            bf16x8 fb[4];
+        for (int ks = 0; ks < W::BM / 32; ++ks) {
+            bf16x8 fb[W::T2];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) fb[b] = tr_frag(bbase + ks * 32 * W8_PITCH + b * 32, W8_PITCH);
+            for (int b = 0; b < W::T2; ++b) fb[b] = tr_frag(buf + boff + ks * 32 * W::PB + b * 32, W::PB);
 #pragma unroll
-            for (int q = 0; q < PLANES; ++q)
+            for (int q = 0; q < W::PLANES; ++q)
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const bf16x8 fa = tr_frag(abase + q * PLANE + ks * 32 * W8_PITCH + a * 32, W8_PITCH);
+                for (int a = 0; a < W::T1; ++a) {
+                    const bf16x8 fa = tr_frag(buf + aoff + q * W::ABYTES + ks * 32 * W::PA + a * 32, W::PA);
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        if constexpr (KIND == SAD_SRC_F16)
-                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, fa), __builtin_bit_cast(f16x8, fb[b]),
-                                                                               acc[a][b], 0, 0, 0);
-                        else acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, fb[b], acc[a][b], 0, 0, 0);
-                    }
+                    for (int b = 0; b < W::T2; ++b) acc[a][b] = mma(fa, fb[b], acc[a][b]);
                 }
+            if (bias) {      // uniform: the waves of a row of the workgroup share its columns
+#pragma unroll
+                for (int q = 0; q < W::PLANES; ++q)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (w2 + j * W::W2 < W::T1)
+                            accb[j] = mma(tr_frag(buf + aoff + q * W::ABYTES + ks * 32 * W::PA + (w2 + j * W::W2) * 32, W::PA), ones, accb[j]);
+            }
+        }
+    };
+
+    issue(0);
+    stage(lds);
+    if (nst > 1) issue(1);
+    __syncthreads();
+    const bool early = wave < W::W1 * W::W2 / 2;
+    for (int s = 0; s < nst; ++s) {
+        unsigned char* cur = lds + (s & 1) * W::BUF;
+        unsigned char* nxt = lds + ((s + 1) & 1) * W::BUF;
+        if (early && s + 1 < nst) {
+            stage(nxt);
+            if (s + 2 < nst) issue(s + 2);
+        }
+        multiply(cur);
+        if (!early && s + 1 < nst) {
+            stage(nxt);
+            if (s + 2 < nst) issue(s + 2);
         }
         __syncthreads();
     }
     float* out = p.out + (long long)split * p.N * p.K;
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
+    for (int a = 0; a < W::T1; ++a)
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int e = 0; e < 4; ++e) {
+            const int n = n0 + w1 * (W::BN / W::W1) + 16 * a + 4 * (lane >> 4) + e, k = k0 + w2 * (W::BK / W::W2) + (lane & 15);
+            if (n < p.N) {
+                float* q = out + (long long)n * p.K + k;
+#pragma unroll
+                for (int b = 0; b < W::T2; ++b)
+                    if (k + 16 * b < p.K) q[16 * b] = acc[a][b][e];
+            }
+        }
+    if (bias && (lane & 15) == 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int n = n0 + w1 * 64 + 16 * a + 4 * (lane >> 4) + e, k = k0 + w2 * 64 + 16 * b + (lane & 15);
-                if (n < p.N && k < p.K) out[(long long)n * p.K + k] = acc[a][b][e];
+                const int a = w2 + j * W::W2, n = n0 + w1 * (W::BN / W::W1) + 16 * a + 4 * (lane >> 4) + e;
+                if (a < W::T1 && n < p.N) p.out_b[(long long)split * p.N + n] = accb[j][e];
             }
-    if (p.out_b != nullptr && k0 == 0) {
-        float* red = (float*)lds;                           // [16 row groups][128 columns]
-#pragma unroll
-        for (int j = 0; j < 8; ++j) red[rr * W8_BN + cc * 8 + j] = bias[j];
-        __syncthreads();
-        if (tid < W8_BN && n0 + tid < p.N) {
-            float s = 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) s += red[j * W8_BN + tid];
-            p.out_b[(long long)split * p.N + n0 + tid] = s;
-        }
     }
 }
 

@@ -973,7 +973,7 @@ def weight_grad8(dy, ckpt, bias=False):
     dy, n0, n1, s0, s1 = _rows2(dy)
     dw = torch.empty((N, K), dtype=torch.float32, device=dev)
     db = torch.empty(N, dtype=torch.float32, device=dev) if bias else None
-    ws = _bytes(dev, "sad_weight_grad8_workspace_bytes", n0 * n1, N, K)
+    ws = _bytes(dev, "sad_weight_grad8_workspace_bytes", n0 * n1, N, K, kind)
     _launch("sad_weight_grad8", dev, n0, n1, N, K, kind, dy.data_ptr(), s0, s1, ckpt.saved.data_ptr(), dw.data_ptr(), _addr(db),
             ws.data_ptr())
     return (dw, db) if bias else dw

@@ -167,7 +167,7 @@ def load():
     lib.sad_checkpoint8_bytes.argtypes = [c_int64] * 2
     lib.sad_checkpoint8_save.argtypes = [c_int64] * 3 + [c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p]
     lib.sad_checkpoint8_restore.argtypes = [c_int64] * 2 + [c_int32, c_void_p, c_void_p, c_void_p]
-    lib.sad_weight_grad8_workspace_bytes.argtypes = [c_int64] * 3
+    lib.sad_weight_grad8_workspace_bytes.argtypes = [c_int64] * 3 + [c_int32]
     lib.sad_weight_grad8.argtypes = [c_int64] * 4 + [c_int32, c_void_p, c_int64, c_int64] + [c_void_p] * 5
     for name in ("sad_gated_scan_workspace_bytes", "sad_gated_scan_kept_bytes", "sad_gated_scan_codes_bytes",
                  "sad_checkpoint8_bytes", "sad_weight_grad8_workspace_bytes"):
