@@ -179,14 +179,17 @@ __global__ __launch_bounds__(W::NT) void k_wgrad8(Wgrad8P p) {
         for (int i = 0; i < W::NB; ++i) {
             const float scale = c8_scale((int)re[i]);
             u32x4 v[2];
+            float low = 0.f;                  // smallest code: -128 where an entry was lost
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const unsigned w = rb[i][j];
-                v[j >> 1][(j & 1) * 2] = c8_pack16(c8_value<0>(w, scale), c8_value<1>(w, scale), KIND == SAD_SRC_F16);
-                v[j >> 1][(j & 1) * 2 + 1] = c8_pack16(c8_value<2>(w, scale), c8_value<3>(w, scale), KIND == SAD_SRC_F16);
+                const float c0 = c8_int<0>(w), c1 = c8_int<1>(w), c2 = c8_int<2>(w), c3 = c8_int<3>(w);
+                low = fminf(fminf(low, c0), c1);
+                low = fminf(fminf(low, c2), c3);
+                v[j >> 1][(j & 1) * 2] = c8_pack16(c0 * scale, c1 * scale, KIND == SAD_SRC_F16);
+                v[j >> 1][(j & 1) * 2 + 1] = c8_pack16(c2 * scale, c3 * scale, KIND == SAD_SRC_F16);
             }
-            const unsigned lost = c8_any_lost(rb[i][0]) | c8_any_lost(rb[i][1]) | c8_any_lost(rb[i][2]) | c8_any_lost(rb[i][3]);
-            if (__any(lost != 0u)) {      // a lost entry's NaN
+            if (__any(low < -127.5f)) {       // a lost entry's NaN
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                     if (((rb[i][j >> 2] >> (8 * (j & 3))) & 0xffu) == C8_LOST) v[j >> 3][(j >> 1) & 3] |= 0x7fffu << (16 * (j & 1));
@@ -227,14 +230,16 @@ __global__ __launch_bounds__(W::NT) void k_wgrad8(Wgrad8P p) {
 #pragma unroll
                     for (int b = 0; b < W::T2; ++b) acc[a][b] = mma(fa, fb[b], acc[a][b]);
                 }
-            if (bias) {      // uniform: the waves of a row of the workgroup share its columns
+        }
+        if (bias) {      // uniform: the waves of a row of the workgroup share its columns
+#pragma unroll
+            for (int ks = 0; ks < W::BM / 32; ++ks)
 #pragma unroll
                 for (int q = 0; q < W::PLANES; ++q)
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
                         if (w2 + j * W::W2 < W::T1)
                             accb[j] = mma(tr_frag(buf + aoff + q * W::ABYTES + ks * 32 * W::PA + (w2 + j * W::W2) * 32, W::PA), ones, accb[j]);
-            }
         }
     };
 
@@ -250,7 +255,9 @@ __global__ __launch_bounds__(W::NT) void k_wgrad8(Wgrad8P p) {
             stage(nxt);
             if (s + 2 < nst) issue(s + 2);
         }
+        __builtin_amdgcn_s_setprio(1);      // the SIMD's other wave is staging
         multiply(cur);
+        __builtin_amdgcn_s_setprio(0);
         if (!early && s + 1 < nst) {
             stage(nxt);
             if (s + 2 < nst) issue(s + 2);
