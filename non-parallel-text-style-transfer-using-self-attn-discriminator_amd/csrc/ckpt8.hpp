@@ -7,7 +7,9 @@
 //     of e below) in fp16: a checkpoint can feed a matrix instruction without a second rounding;
 //   * a power-of-two step costs up to one bit against a free scale (64..127 codes used on each side) and makes encode
 //     and decode exact but for the one rounding to the code: error <= 2^e / 2 per entry;
-//   * code -128 marks a non-finite entry: it comes back as NaN, its 31 neighbours are not touched;
+//   * code -128 marks a non-finite entry: it comes back as NaN, its 31 neighbours are not touched.  A block that holds one
+//     has the exponent byte 255 and its exponent in a second array, which is neither written nor read otherwise: readers
+//     test one byte per block instead of every code;
 //   * e is clamped to [-126, 122] (fp16: [-24, 10]).  At the upper end the code stops at +-63, where 64 would restore
 //     to infinity; at the lower end 2^e stays a normal float (fp16: the spacing of its subnormals).
 #pragma once
@@ -44,11 +46,7 @@ __device__ __forceinline__ unsigned c8_code(float x, float inv, float cap) {
     return (unsigned)(int)q & 0xffu;
 }
 constexpr unsigned C8_LOST = 0x80u;                // code of a non-finite entry
-// any of the four codes of w lost?
-__device__ __forceinline__ unsigned c8_any_lost(unsigned w) {
-    w ^= 0x80808080u;
-    return (w - 0x01010101u) & ~w & 0x80808080u;
-}
+constexpr unsigned C8_MARK = 255u;                 // exponent byte of a block that holds one
 // code N of w: one conversion with a sign-extended byte operand (from C++ the compiler makes two or three instructions)
 template <int N>
 __device__ __forceinline__ float c8_int(unsigned w) {
@@ -130,7 +128,8 @@ __device__ __forceinline__ void c8_load16(float (&v)[16], const void* row, int c
 // types move 3.06 bytes per element each way.
 template <int KIND>
 __global__ __launch_bounds__(256) void k_ckpt8_save(int rows, int C, int per, int rpb, const void* __restrict__ x, Rows2 xr,
-                                                   unsigned char* __restrict__ codes, unsigned char* __restrict__ exps) {
+                                                   unsigned char* __restrict__ codes, unsigned char* __restrict__ exps,
+                                                   unsigned char* __restrict__ marked) {
     const int r = (int)threadIdx.x / per, row = blockIdx.x * rpb + r;
     if (r >= rpb && rpb > 1) return;
     if (row >= rows) return;
@@ -164,33 +163,53 @@ __global__ __launch_bounds__(256) void k_ckpt8_save(int rows, int C, int per, in
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[k] |= c8_code(v[4 * k + i], inv, cap) << (8 * i);
         }
+        const unsigned pair = (unsigned)__builtin_amdgcn_update_dpp(0, (int)all, 0xB1, 0xf, 0xf, false);
+        const bool lost = all >= C8_NONFINITE || pair >= C8_NONFINITE;
         if (all >= C8_NONFINITE) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (c8_abs_bits(v[i]) >= C8_NONFINITE) w[i >> 2] = (w[i >> 2] & ~(0xffu << (8 * (i & 3)))) | (C8_LOST << (8 * (i & 3)));
         }
         *(u32x4*)(codes + ((long long)row * per + q) * 16) = w;
-        if ((q & 1) == 0) exps[(long long)row * (per >> 1) + (q >> 1)] = (unsigned char)e;
+        if ((q & 1) == 0) {
+            const long long at = (long long)row * (per >> 1) + (q >> 1);
+            exps[at] = lost ? (unsigned char)C8_MARK : (unsigned char)e;
+            if (lost) marked[at] = (unsigned char)e;
+        }
     }
 }
 
 template <int KIND>
 __global__ __launch_bounds__(256) void k_ckpt8_restore(int rows, int C, int per, int rpb, const unsigned char* __restrict__ codes,
-                                                      const unsigned char* __restrict__ exps, void* __restrict__ out) {
+                                                      const unsigned char* __restrict__ exps,
+                                                      const unsigned char* __restrict__ marked, void* __restrict__ out) {
     const int r = (int)threadIdx.x / per, row = blockIdx.x * rpb + r;
     if (r >= rpb && rpb > 1) return;
     if (row >= rows) return;
     char* op = (char*)out + (long long)row * C * Elem<KIND>::bytes;
     for (int q = rpb > 1 ? (int)threadIdx.x - r * per : (int)threadIdx.x; q < per; q += 256) {
         const u32x4 w = *(const u32x4*)(codes + ((long long)row * per + q) * 16);
-        const float scale = c8_scale(exps[(long long)row * (per >> 1) + (q >> 1)]);
+        const long long at = (long long)row * (per >> 1) + (q >> 1);
+        const unsigned byte = exps[at];
         float v[16];
+        if (byte != C8_MARK) {
+            const float scale = c8_scale((int)byte);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            v[4 * k + 0] = c8_value_checked<0>(w[k], scale);
-            v[4 * k + 1] = c8_value_checked<1>(w[k], scale);
-            v[4 * k + 2] = c8_value_checked<2>(w[k], scale);
-            v[4 * k + 3] = c8_value_checked<3>(w[k], scale);
+            for (int k = 0; k < 4; ++k) {
+                v[4 * k + 0] = c8_value<0>(w[k], scale);
+                v[4 * k + 1] = c8_value<1>(w[k], scale);
+                v[4 * k + 2] = c8_value<2>(w[k], scale);
+                v[4 * k + 3] = c8_value<3>(w[k], scale);
+            }
+        } else {
+            const float scale = c8_scale((int)marked[at]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[4 * k + 0] = c8_value_checked<0>(w[k], scale);
+                v[4 * k + 1] = c8_value_checked<1>(w[k], scale);
+                v[4 * k + 2] = c8_value_checked<2>(w[k], scale);
+                v[4 * k + 3] = c8_value_checked<3>(w[k], scale);
+            }
         }
         const int c = q * 16;
         if (c + 16 <= C) {

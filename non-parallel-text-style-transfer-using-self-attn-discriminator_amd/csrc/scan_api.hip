@@ -153,16 +153,17 @@ int check_matrix(int64_t rows, int64_t C, int kind) {
 }
 
 // ---- weight gradient --------------------------------------------------------------------------------------------------
-// Tile and row splits by an estimate of the time: rounds of workgroups over the 256 CUs, each round as long as its rows
-// take at the tile's rate, and the slab of the splits once written and once read.  Rates measured on [16384, 6144, 2048]
-// and [32768, 1536, 300]: see k_wgrad8.
+// Tile and row splits by an estimate of the time: rounds of workgroups over the 256 CUs, each as long as its rows take at
+// the tile's pace and a fixed start and end, and the slab of the splits, written and read once.  Paces measured in bf16 on
+// [16384 rows, 6144, 2048]: 539 us with 256 x 256 tiles (192 of them), 487 with 192 x 256 (256), 664 with 128 x 320 (336, three
+// splits), 738 with 128 x 128 (768); on [32768, 1536, 300] the same tiles take 71, 67, 55 and 100 us.
 struct Split { int bn, bk, tn, tk, splits, rows; };
 Split wgrad8_split(int64_t M, int64_t N, int64_t K, int kind) {
-    struct Tile { int bn, bk; double us_per_row; };        // time of one workgroup per token row
-    static const Tile wide[] = {{256, 256, 0.0140}, {192, 256, 0.0115}, {128, 128, 0.0065}};
-    static const Tile fp32[] = {{128, 128, 0.0180}};
+    struct Tile { int bn, bk; double us_per_row; };        // pace: time of a workgroup per token row, all CUs at work
+    static const Tile wide[] = {{256, 256, 0.0325}, {192, 256, 0.0295}, {128, 320, 0.0285}, {128, 128, 0.0150}};
+    static const Tile fp32[] = {{128, 128, 0.0400}};
     const Tile* t = kind == SAD_SRC_F32 ? fp32 : wide;
-    const int nt = kind == SAD_SRC_F32 ? 1 : 3;
+    const int nt = kind == SAD_SRC_F32 ? 1 : 4;
     Split best{};
     double best_us = 1e30;
     for (int i = 0; i < nt; ++i) {
@@ -174,7 +175,7 @@ Split wgrad8_split(int64_t M, int64_t N, int64_t K, int kind) {
             if (splits != n && n > 1) continue;
             if (n > 1 && rows < 256) break;
             const int64_t rounds = (tn * tk * splits + 255) / 256;
-            const double us = 3.0 + rounds * (rows * t[i].us_per_row + 2.0) + (splits > 1 ? 3.0 + (splits + 1.0) * 2 * 4 * N * K / 4.0e6 : 0.0);
+            const double us = rounds * (rows * t[i].us_per_row + 5.0) + (splits > 1 ? 3.0 + splits * 8.0 * N * K / 4.0e6 : 0.0);
             if (us < best_us) {
                 best_us = us;
                 best = Split{t[i].bn, t[i].bk, (int)tn, (int)tk, (int)splits, (int)rows};
@@ -198,6 +199,7 @@ int launch_wgrad8(const Wgrad8P& p, const Split& s, hipStream_t st) {
     if constexpr (KIND != SAD_SRC_F32) {
         if (s.bn == 256) return launch_wgrad8<KIND, 256, 256, 2, 4>(p, st);
         if (s.bn == 192) return launch_wgrad8<KIND, 192, 256, 2, 4>(p, st);
+        if (s.bk == 320) return launch_wgrad8<KIND, 128, 320, 2, 4>(p, st);
     }
     return launch_wgrad8<KIND, 128, 128, 2, 2>(p, st);
 }
@@ -273,7 +275,7 @@ int sad_gated_scan_step(int32_t B, int32_t D, int32_t kind, int32_t gated, const
 size_t sad_checkpoint8_bytes(int64_t rows, int64_t C) {
     if (check_matrix(rows, C, SAD_SRC_F32)) return 0;
     const size_t nb = (size_t)((C + C8_BLOCK - 1) / C8_BLOCK);
-    return (size_t)rows * nb * (C8_BLOCK + 1);
+    return (size_t)rows * nb * (C8_BLOCK + 2);        // codes, exponents, exponents of marked blocks
 }
 
 int sad_checkpoint8_save(int64_t n0, int64_t n1, int64_t C, int32_t kind, const void* x, int64_t stride0, int64_t stride1,
@@ -290,7 +292,7 @@ int sad_checkpoint8_save(int64_t n0, int64_t n1, int64_t C, int32_t kind, const 
     unsigned char* exps = codes + (size_t)rows * nb * C8_BLOCK;
     const Rows2 xr{stride0, stride1, (unsigned)n1};
     BY_KIND(kind, hipLaunchKernelGGL((k_ckpt8_save<KIND>), dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, (hipStream_t)stream,
-                                     (int)rows, (int)C, per, rpb, x, xr, codes, exps));
+                                     (int)rows, (int)C, per, rpb, x, xr, codes, exps, exps + (size_t)rows * nb));
     SAD_LAUNCHED("k_ckpt8_save");
     return 0;
 }
@@ -304,7 +306,7 @@ int sad_checkpoint8_restore(int64_t rows, int64_t C, int32_t kind, const void* s
     const unsigned char* codes = (const unsigned char*)saved;
     const unsigned char* exps = codes + (size_t)rows * nb * C8_BLOCK;
     BY_KIND(kind, hipLaunchKernelGGL((k_ckpt8_restore<KIND>), dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0,
-                                     (hipStream_t)stream, (int)rows, (int)C, per, rpb, codes, exps, out));
+                                     (hipStream_t)stream, (int)rows, (int)C, per, rpb, codes, exps, exps + (size_t)rows * nb, out));
     SAD_LAUNCHED("k_ckpt8_restore");
     return 0;
 }
@@ -338,28 +340,24 @@ int sad_weight_grad8(int64_t n0, int64_t n1, int64_t N, int64_t K, int32_t kind,
     // Chunks of 8 columns reach `over` entries past a row's end where N is no multiple of 8: memory of the rows behind, which
     // is there for all rows but the last few.
     const int64_t over = (8 - N % 8) % 8;
-    p.fast_rows = !p.y_flat ? 0 : (over == 0 ? (int)M : (stride1 > 0 ? (int)(M - (over + stride1 - 1) / stride1) : 0));
+    p.fast_rows = !p.y_flat || stride1 > (1 << 22) ? 0 : (over == 0 ? (int)M : (stride1 > 0 ? (int)(M - (over + stride1 - 1) / stride1) : 0));
     p.codes = (const unsigned char*)saved;
     p.exps = p.codes + (size_t)M * p.Kp;
+    p.marked = p.exps + (size_t)M * (p.Kp / C8_BLOCK);
     p.per_xcd = (int)((groups + 7) / 8);
     p.tn = s.tn; p.tk = s.tk; p.splits = s.splits; p.rows = s.rows;
-    float* part_b = (float*)workspace + (size_t)s.splits * N * K;
     p.out = s.splits > 1 ? (float*)workspace : dw;
-    p.out_b = db == nullptr ? nullptr : (s.splits > 1 ? part_b : db);
+    p.out_b = db == nullptr ? nullptr : (s.splits > 1 ? p.out + N * K : db);
+    p.slab = N * K + N;
     hipStream_t st = (hipStream_t)stream;
     int rc = 0;
     BY_KIND(kind, rc = launch_wgrad8<KIND>(p, s, st));
     if (rc != 0) return rc;
     if (s.splits > 1) {
-        const long long n = (long long)N * K;
-        long long g = (n + 255) / 256;
-        hipLaunchKernelGGL(k_wgrad8_join, dim3((unsigned)(g < 8192 ? g : 8192)), dim3(256), 0, st, n, s.splits, (const float*)workspace, dw);
+        const long long n = db == nullptr ? (long long)N * K : p.slab, g = (n + 255) / 256;
+        hipLaunchKernelGGL(k_wgrad8_join, dim3((unsigned)(g < 8192 ? g : 8192)), dim3(256), 0, st, n, (long long)N * K, s.splits, p.slab,
+                           (const float*)workspace, dw, db);
         SAD_LAUNCHED("k_wgrad8_join");
-        if (db != nullptr) {
-            hipLaunchKernelGGL(k_wgrad8_join, dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, (long long)N, s.splits,
-                               (const float*)part_b, db);
-            SAD_LAUNCHED("k_wgrad8_join");
-        }
     }
     return 0;
 }
