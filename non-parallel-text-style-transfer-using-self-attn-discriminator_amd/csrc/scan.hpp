@@ -30,6 +30,9 @@ namespace sad {
 constexpr int SC_STEPS = 16;       // time steps of a block: states kept, loads in flight
 constexpr int SC_CH = 128;         // channels of a wave
 constexpr int SC_GROUP = 4;        // time chunks whose maps one workgroup joins
+// how a block is computed: every step valid; every row inside the tensor, steps behind the sentence masked by selects; rows
+// past the end of the tensor
+constexpr int SC_FULL = 2, SC_INSIDE = 1, SC_EDGE = 0;
 constexpr float SC_LOG2E = 1.4426950408889634f;
 
 struct ScanP {
@@ -211,6 +214,16 @@ __device__ __forceinline__ void scan_leave(const ScanP& p, const ScanAt& w, f32x
     }
 }
 
+template <class F> __device__ __forceinline__ void sc_by_mode(int mode, F&& f) {
+    if (mode == SC_FULL) f(std::integral_constant<int, SC_FULL>{});
+    else if (mode == SC_INSIDE) f(std::integral_constant<int, SC_INSIDE>{});
+    else f(std::integral_constant<int, SC_EDGE>{});
+}
+__device__ __forceinline__ int sc_mode(int kb, int len, int T) {
+    return (kb + 1) * SC_STEPS <= len ? SC_FULL : ((kb + 1) * SC_STEPS <= T ? SC_INSIDE : SC_EDGE);
+}
+__device__ __forceinline__ f32x2 sc_select(bool c, f32x2 a, f32x2 b) { return f32x2{c ? a[0] : b[0], c ? a[1] : b[1]}; }
+
 // A lane's 32-bit offset, opaque from here on: its zero extension then stays in the block of code that uses it, where
 // scalar base + lane offset is one address operand; hoisted out of a loop it costs a 64-bit vector addition per access.
 __device__ __forceinline__ unsigned sc_here(unsigned v) {
@@ -378,31 +391,30 @@ __global__ __launch_bounds__(256) void k_scan_fwd(ScanP p) {
             }
             if (lane == 0) p.lost[((long long)w.b * p.nblk + kb) * p.ncg + w.cg] = lost ? 1u : 0u;
         }
-        auto block = [&](auto full) {
+        sc_by_mode(sc_mode(kb, w.len, p.T), [&](auto mode) {
+            constexpr int MODE = decltype(mode)::value;
             unsigned char* yr = yb + (long long)(kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 : 0)) * yst;
             const unsigned vy = sc_here(voff[0]);
 #pragma unroll
             for (int i = 0; i < SC_STEPS; ++i) {
                 const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-                const bool ok = decltype(full)::value || t < w.len;
+                const bool ok = MODE == SC_FULL || t < w.len;
                 const f32x2 xv = Pair<KIND>::get(z[0][i]), fv = Pair<KIND>::get(z[1][i]);
                 f32x2 hn;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) hn[e] = __builtin_fmaf(sc_share(fv[e]), xv[e] - h[e], h[e]);
-                if (ok) h = hn;                                     // uniform
+                h = sc_select(ok, hn, h);
                 f32x2 yv = h;
                 if constexpr (GATED) {
                     const f32x2 ov = Pair<KIND>::get(z[PARTS - 1][i]);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) yv[e] = h[e] * sigmoidf_(ov[e]);
                 }
-                if (!ok) yv = f32x2{0.f, 0.f};
-                if (decltype(full)::value || t < p.T) Pair<KIND>::store(yr + vy, yv);
+                yv = sc_select(ok, yv, f32x2{0.f, 0.f});
+                if (MODE != SC_EDGE || t < p.T) Pair<KIND>::store(yr + vy, yv);
                 yr += p.reverse ? -yst : yst;
             }
-        };
-        if ((kb + 1) * SC_STEPS <= w.len) block(std::integral_constant<bool, true>{});
-        else block(std::integral_constant<bool, false>{});
+        });
     }
     if (w.ord == p.nchunk - 1) *(f32x2u*)(p.h_last + (long long)w.b * p.D + w.cc) = h;
 }
@@ -431,13 +443,12 @@ __global__ __launch_bounds__(64 * SC_GROUP) void k_scan_sum(ScanP p) {
         for (int i = 0; i < SC_STEPS; ++i) {
             const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
             const f32x2 xv = Pair<KIND>::get(z[0][i]), fv = Pair<KIND>::get(z[1][i]);
-            if (t < w.len) {                                        // uniform
+            const bool ok = t < w.len;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float s = sc_share(fv[e]);
-                    h[e] = __builtin_fmaf(s, xv[e] - h[e], h[e]);
-                    m[e] = __builtin_fmaf(s, 1.0f - m[e], m[e]);
-                }
+            for (int e = 0; e < 2; ++e) {
+                const float s = sc_share(fv[e]);
+                h[e] = ok ? __builtin_fmaf(s, xv[e] - h[e], h[e]) : h[e];
+                m[e] = ok ? __builtin_fmaf(s, 1.0f - m[e], m[e]) : m[e];
             }
         }
     }
@@ -568,27 +579,28 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanP p) {
             for (int i = 0; i < SC_STEPS; ++i) dy[0][i] = Pair<KIND>::zero();
         }
         __builtin_amdgcn_sched_barrier(0);
-        const bool full_block = (kb + 1) * SC_STEPS <= w.len && !in.lost();
+        // lost entries are looked for in the slowest form only
+        const int mode = in.lost() ? SC_EDGE : sc_mode(kb, w.len, p.T);
         f32x2 h[SC_STEPS], odds[SC_STEPS];                          // states; e^f
-        auto states = [&](auto full) {
-            constexpr bool FULL = decltype(full)::value;
+        auto states = [&](auto m) {
+            constexpr int MODE = decltype(m)::value;
             f32x2 hc = enter;
             static_for<SC_STEPS>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-                const f32x2 fa = in.template times<1, i, !FULL>(SC_LOG2E), xd = in.template x_less<i, !FULL>(hc);
+                const f32x2 fa = in.template times<1, i, MODE == SC_EDGE>(SC_LOG2E), xd = in.template x_less<i, MODE == SC_EDGE>(hc);
                 f32x2 hn;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     odds[i][e] = sc_odds(fa[e]);
                     hn[e] = __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + odds[i][e]), xd[e], hc[e]);
                 }
-                if (FULL || t < w.len) hc = hn;                     // uniform
+                hc = sc_select(MODE == SC_FULL || t < w.len, hn, hc);
                 h[i] = hc;
             });
         };
-        auto grads = [&](auto full) {
-            constexpr bool FULL = decltype(full)::value;
+        auto grads = [&](auto m) {
+            constexpr int MODE = decltype(m)::value;
             unsigned char* gr = gb + (long long)(kb * SC_STEPS + (p.reverse ? 0 : SC_STEPS - 1)) * dzst;
             unsigned vg[PARTS];
 #pragma unroll
@@ -596,11 +608,11 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanP p) {
             static_for<SC_STEPS>([&](auto jc) {
                 constexpr int i = SC_STEPS - 1 - decltype(jc)::value;
                 const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-                const bool ok = FULL || t < w.len;
+                const bool ok = MODE == SC_FULL || t < w.len;
                 const f32x2 hp = i == 0 ? enter : h[i == 0 ? 0 : i - 1], dyv = Pair<KIND>::get(dy[0][i]);
-                const f32x2 xd = in.template x_less<i, !FULL>(hp);
+                const f32x2 xd = in.template x_less<i, MODE == SC_EDGE>(hp);
                 f32x2 oa, dx, df, dov, cn;
-                if constexpr (GATED) oa = in.template times<PARTS - 1, i, !FULL>(-SC_LOG2E);
+                if constexpr (GATED) oa = in.template times<PARTS - 1, i, MODE == SC_EDGE>(-SC_LOG2E);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float dh = dyv[e];
@@ -614,9 +626,12 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanP p) {
                     df[e] = -(odds[i][e] * sv * dx[e]) * xd[e];
                     cn[e] = __builtin_fmaf(-sv, g, g);
                 }
-                if (ok) carry = cn;                                 // uniform
-                else dx = df = dov = f32x2{0.f, 0.f};
-                if (FULL || t < p.T) {
+                const f32x2 none{0.f, 0.f};
+                carry = sc_select(ok, cn, carry);
+                dx = sc_select(ok, dx, none);
+                df = sc_select(ok, df, none);
+                if constexpr (GATED) dov = sc_select(ok, dov, none);
+                if (MODE != SC_EDGE || t < p.T) {
                     Pair<KIND>::store(gr + vg[0], dx);
                     Pair<KIND>::store(gr + vg[1], df);
                     if constexpr (GATED) Pair<KIND>::store(gr + vg[PARTS - 1], dov);
@@ -624,13 +639,11 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanP p) {
                 gr += p.reverse ? dzst : -dzst;
             });
         };
-        if (full_block) states(std::integral_constant<bool, true>{});
-        else states(std::integral_constant<bool, false>{});
+        sc_by_mode(mode, states);
         __builtin_amdgcn_sched_barrier(0);
         in.forget();
         if (it + 1 < n) issue(p.reverse ? kb + 1 : kb - 1);
-        if (full_block) grads(std::integral_constant<bool, true>{});
-        else grads(std::integral_constant<bool, false>{});
+        sc_by_mode(mode, grads);
     }
     if (p.dh0 != nullptr && w.ord == p.nchunk - 1) *(f32x2u*)(p.dh0 + (long long)w.b * p.D + w.cc) = carry;
 }
@@ -671,18 +684,17 @@ __global__ __launch_bounds__(64 * SC_GROUP) void k_scan_bsum(ScanP p) {
             static_for<SC_STEPS>([&](auto jc) {
                 constexpr int i = SC_STEPS - 1 - decltype(jc)::value;
                 const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-                if (t < w.len) {                                    // uniform
-                    const f32x2 fa = in.template times<1, i, CHECKED>(SC_LOG2E), dyv = Pair<KIND>::get(dy[i]);
-                    f32x2 oa;
-                    if constexpr (GATED) oa = in.template times<PARTS - 1, i, CHECKED>(-SC_LOG2E);
+                const bool ok = t < w.len;
+                const f32x2 fa = in.template times<1, i, CHECKED>(SC_LOG2E), dyv = Pair<KIND>::get(dy[i]);
+                f32x2 oa;
+                if constexpr (GATED) oa = in.template times<PARTS - 1, i, CHECKED>(-SC_LOG2E);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float dh = dyv[e];
-                        if constexpr (GATED) dh *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(oa[e]));
-                        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fa[e])), g = dh + v[e];
-                        v[e] = __builtin_fmaf(-s, g, g);
-                        m[e] = __builtin_fmaf(s, 1.0f - m[e], m[e]);
-                    }
+                for (int e = 0; e < 2; ++e) {
+                    float dh = dyv[e];
+                    if constexpr (GATED) dh *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(oa[e]));
+                    const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fa[e])), g = dh + v[e];
+                    v[e] = ok ? __builtin_fmaf(-s, g, g) : v[e];
+                    m[e] = ok ? __builtin_fmaf(s, 1.0f - m[e], m[e]) : m[e];
                 }
             });
         };

@@ -428,6 +428,12 @@ def test_linear8(dtype, bias):
     assert gd.dtype == dt and torch.equal(gd, grads[1].to(dt))
     gx, = torch.autograd.grad(Fn.linear8(x, w.detach(), b.detach() if bias else None), x, dy)
     assert torch.equal(gx, grads[0])
+    with torch.no_grad():
+        plain = Fn.linear8(x, w, b)
+    assert not plain.requires_grad and torch.equal(plain, y) and plain.stride() == y.stride()
+    one = Fn.linear8(xf[0, 0], wd)
+    g1, = torch.autograd.grad(one, wd, dy[0, 0])
+    assert tuple(one.shape) == (N,) and g1.abs().max() > 0
 
 
 # ---- the operators together ------------------------------------------------------------------------------------------
