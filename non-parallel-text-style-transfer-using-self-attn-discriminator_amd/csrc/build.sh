@@ -21,6 +21,15 @@ for src in sad_api scan_api; do
         -o "$OBJ/$src.o" "$HERE/$src.hip" &
     pids+=($!)
 done
+# Autograd nodes for torch's dispatcher (plain C++ against torch's headers; not built for a renamed library)
+if [ -z "${SAD_OUT:-}" ]; then
+    TORCH="$(python3 -c 'import importlib.util, os; print(os.path.dirname(importlib.util.find_spec("torch").origin))')"
+    "${CXX:-g++}" -O2 -std=c++17 -fPIC -shared -Wall -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 \
+        -I"$TORCH/include" -I"$TORCH/include/torch/csrc/api/include" -I"${ROCM_PATH:-/opt/rocm}/include" \
+        -o "$OUT/libsad_torch.so" "$HERE/torch_ops.cpp" \
+        -L"$TORCH/lib" -ltorch -ltorch_cpu -ltorch_hip -lc10 -lc10_hip &
+    pids+=($!)
+fi
 for pid in "${pids[@]}"; do wait "$pid"; done
 "$HIPCC" --offload-arch=gfx950 -shared -fPIC -o "$LIB" "$OBJ/sad_api.o" "$OBJ/scan_api.o"
 echo "built $LIB"

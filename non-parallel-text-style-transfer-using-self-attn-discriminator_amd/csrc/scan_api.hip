@@ -150,7 +150,7 @@ int launch_scan_bwd(const sad_scan_args* a, const ScanP& p, hipStream_t st) {
 // ---- checkpoints ----------------------------------------------------------------------------------------------------
 int check_matrix(int64_t rows, int64_t C, int kind) {
     if (rows < 1 || C < 1) return set_error(-1, "rows and channels must be positive (rows=%lld C=%lld)", (long long)rows, (long long)C);
-    if (rows > MAX_GRID || C > (1 << 24)) return set_error(-1, "rows=%lld or C=%lld beyond the supported maximum", (long long)rows, (long long)C);
+    if (rows > (1 << 30) || C > (1 << 24)) return set_error(-1, "rows=%lld or C=%lld beyond the supported maximum", (long long)rows, (long long)C);
     if (!known_kind(kind)) return set_error(-1, "kind must be SAD_SRC_F32, SAD_SRC_BF16 or SAD_SRC_F16, got %d", kind);
     return 0;
 }

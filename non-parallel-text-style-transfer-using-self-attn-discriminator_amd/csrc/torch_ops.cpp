@@ -1,0 +1,263 @@
+// Autograd nodes of the gated scan and of linear8 for torch's dispatcher (torch.ops.sad_amd.*).
+//
+// functional.py checks the arguments and calls these; they allocate, fill the argument structs and launch through libsad's
+// C-ABI.  They are here and not in Python because the calls are short: the backward pass runs on autograd's device thread,
+// where a Python node first has to take the interpreter lock from the thread that waits for it.
+//
+// The library's functions are handed in as addresses (sad_amd::bind), so this file does not link libsad and follows whichever
+// build of it the package loaded.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/library.h>
+
+#include "../../include/sad.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+struct Api {
+    decltype(&sad_last_error) last_error = nullptr;
+    decltype(&sad_gated_scan_workspace_bytes) scan_ws = nullptr;
+    decltype(&sad_gated_scan_kept_bytes) scan_kept = nullptr;
+    decltype(&sad_gated_scan_codes_bytes) scan_codes = nullptr;
+    decltype(&sad_gated_scan_fwd) scan_fwd = nullptr;
+    decltype(&sad_gated_scan_bwd) scan_bwd = nullptr;
+    decltype(&sad_checkpoint8_bytes) ckpt_bytes = nullptr;
+    decltype(&sad_checkpoint8_save) ckpt_save = nullptr;
+    decltype(&sad_weight_grad8_workspace_bytes) wgrad_ws = nullptr;
+    decltype(&sad_weight_grad8) wgrad = nullptr;
+} api;
+
+// addresses in the order of Api's members
+void bind(at::IntArrayRef a) {
+    TORCH_CHECK(a.size() == 10, "expected 10 addresses");
+    int i = 0;
+    auto take = [&](auto& f) { f = reinterpret_cast<std::decay_t<decltype(f)>>(a[i++]); };
+    take(api.last_error); take(api.scan_ws); take(api.scan_kept); take(api.scan_codes); take(api.scan_fwd); take(api.scan_bwd);
+    take(api.ckpt_bytes); take(api.ckpt_save); take(api.wgrad_ws); take(api.wgrad);
+}
+
+void check(int rc, const char* what) { TORCH_CHECK(rc == 0, "libsad ", what, " failed (", rc, "): ", api.last_error()); }
+size_t size_of(size_t n, const char* what) {
+    TORCH_CHECK(n != 0, "libsad ", what, " failed: ", api.last_error());
+    return n;
+}
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
+int kind_of(at::ScalarType t) { return t == at::kFloat ? SAD_SRC_F32 : (t == at::kBFloat16 ? SAD_SRC_BF16 : SAD_SRC_F16); }
+template <class T> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+
+// autograd.Function's once_differentiable: with create_graph the results raise when they are differentiated again
+variable_list once(variable_list grads, const char* name) {
+    if (!at::GradMode::is_enabled()) return grads;
+    auto fn = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " has no second derivative", (int64_t)grads.size());
+    for (auto& g : grads)
+        if (g.defined()) { g = g.detach(); g.requires_grad_(true); }
+    return (*fn)(std::move(grads));
+}
+
+// ---- gated scan -------------------------------------------------------------------------------------------------------
+struct ScanShape {
+    int64_t B, T, D, ws, kept, codes;
+};
+ScanShape scan_shape(const Tensor& z, bool gated) {
+    ScanShape s;
+    s.B = z.size(0); s.T = z.size(1); s.D = z.size(2) / (gated ? 3 : 2);
+    s.ws = (int64_t)size_of(api.scan_ws((int)s.B, (int)s.T, (int)s.D), "sad_gated_scan_workspace_bytes");
+    s.kept = ((int64_t)api.scan_kept((int)s.B, (int)s.T, (int)s.D) + 15) / 16 * 16;
+    s.codes = (int64_t)api.scan_codes((int)s.B, (int)s.T, (int)s.D, gated);
+    return s;
+}
+
+// (y, h_last, kept states and behind them the codes)
+std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& z, const Tensor& h0, const Tensor& lengths, bool reverse, bool gated,
+                                                bool int8, bool track) {
+    const c10::DeviceGuard guard(z.device());
+    const ScanShape s = scan_shape(z, gated);
+    Tensor y;
+    if (s.B > 1 && s.T > 1 && z.stride(0) < z.stride(1)) y = at::empty({s.T, s.B, s.D}, z.options()).transpose(0, 1);
+    else y = at::empty({s.B, s.T, s.D}, z.options());
+    Tensor h_last = at::empty({s.B, s.D}, z.options().dtype(at::kFloat)), kept;
+    if (track) kept = bytes(s.kept + (int8 ? s.codes : 0), z);
+    const Tensor ws = s.ws > 16 ? bytes(s.ws, z) : h_last;      // any address where none is needed
+    sad_scan_args a{};
+    a.B = (int)s.B; a.T = (int)s.T; a.D = (int)s.D;
+    a.kind = kind_of(z.scalar_type()); a.gated = gated; a.reverse = reverse;
+    a.z = z.data_ptr(); a.z_stride_b = z.stride(0); a.z_stride_t = z.stride(1);
+    a.lengths = ptr<int32_t>(lengths);
+    a.h0 = ptr<float>(h0);
+    a.y = y.data_ptr(); a.y_stride_b = y.stride(0); a.y_stride_t = y.stride(1);
+    a.h_last = ptr<float>(h_last);
+    if (track) {
+        a.kept = ptr<float>(kept);
+        if (int8) a.codes = ptr<char>(kept) + s.kept;
+    }
+    check(api.scan_fwd(&a, ws.data_ptr(), stream_of(z)), "sad_gated_scan_fwd");
+    return {y, h_last, kept};
+}
+
+bool is_dense(at::IntArrayRef size, at::IntArrayRef stride) {      // a permutation of a contiguous [.., .., C]
+    if (stride[2] != 1) return false;
+    const int a = stride[0] < stride[1] ? 0 : 1, b = 1 - a;
+    return (size[a] == 1 || stride[a] == size[2]) && (size[b] == 1 || stride[b] == size[2] * size[a]);
+}
+
+struct GatedScan : torch::autograd::Function<GatedScan> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& z, const OptTensor& h0, const OptTensor& lengths, bool reverse,
+                                 bool gated, bool int8) {
+        const Tensor l = lengths.value_or(Tensor());
+        auto [y, h_last, kept] = scan_forward(z, h0.value_or(Tensor()), l, reverse, gated, int8, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({int8 ? Tensor() : z, l, kept});
+        ctx->saved_data["s"] = std::vector<int64_t>{z.size(0), z.size(1), z.size(2), z.stride(0), z.stride(1), z.stride(2),
+                                                    (int64_t)z.scalar_type(), reverse, gated, h0.has_value()};
+        return {y, h_last};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list gout) {
+        Tensor dy = gout[0], dh = gout[1];
+        if (!dy.defined() && !dh.defined()) return variable_list(6);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &z = saved[0], &lengths = saved[1], &kept = saved[2];
+        const auto v = ctx->saved_data["s"].toIntVector();
+        const bool reverse = v[7] != 0, gated = v[8] != 0;
+        const c10::DeviceGuard guard(kept.device());
+        const auto options = kept.options().dtype((at::ScalarType)v[6]);
+        const at::IntArrayRef size(v.data(), 3), stride(v.data() + 3, 3);
+        Tensor dz = is_dense(size, stride) ? at::empty_strided(size, stride, options) : at::empty(size, options), dh0;
+        const ScanShape s = scan_shape(dz, gated);
+        if (dy.defined() && dy.stride(2) != 1) dy = dy.contiguous();
+        if (dh.defined()) dh = dh.contiguous();
+        if (v[9] && ctx->needs_input_grad(1)) dh0 = at::empty({s.B, s.D}, options.dtype(at::kFloat));
+        const Tensor ws = s.ws > 16 ? bytes(s.ws, kept) : dz;
+        sad_scan_args a{};
+        a.B = (int)s.B; a.T = (int)s.T; a.D = (int)s.D;
+        a.kind = kind_of(dz.scalar_type()); a.gated = gated; a.reverse = reverse;
+        a.lengths = ptr<int32_t>(lengths);
+        a.kept = ptr<float>(kept);
+        if (z.defined()) { a.z = z.data_ptr(); a.z_stride_b = stride[0]; a.z_stride_t = stride[1]; }
+        else a.codes = ptr<char>(kept) + s.kept;
+        if (dy.defined()) { a.dy = dy.data_ptr(); a.dy_stride_b = dy.stride(0); a.dy_stride_t = dy.stride(1); }
+        a.dh_last = ptr<float>(dh);
+        a.dz = dz.data_ptr(); a.dz_stride_b = dz.stride(0); a.dz_stride_t = dz.stride(1);
+        a.dh0 = ptr<float>(dh0);
+        check(api.scan_bwd(&a, ws.data_ptr(), stream_of(kept)), "sad_gated_scan_bwd");
+        if (!ctx->needs_input_grad(0)) dz = Tensor();
+        return once({dz, dh0, Tensor(), Tensor(), Tensor(), Tensor()}, "gated_scan");
+    }
+};
+
+std::tuple<Tensor, Tensor> gated_scan(const Tensor& z, const OptTensor& h0, const OptTensor& lengths, bool reverse, bool gated, bool int8) {
+    if (at::GradMode::is_enabled() && (z.requires_grad() || (h0.has_value() && h0->requires_grad()))) {
+        auto r = GatedScan::apply(z, h0, lengths, reverse, gated, int8);
+        return {r[0], r[1]};
+    }
+    auto [y, h_last, kept] = scan_forward(z, h0.value_or(Tensor()), lengths.value_or(Tensor()), reverse, gated, false, false);
+    return {y, h_last};
+}
+
+// ---- linear8 ------------------------------------------------------------------------------------------------------------
+struct Rows {
+    Tensor t;      // holds the memory
+    int64_t n0, n1, s0, s1, C;
+};
+// the rows of t [..., C] in their order, without a copy where two strides say it
+Rows rows_of(Tensor t) {
+    if (t.dim() == 1) t = t.unsqueeze(0);
+    if (t.stride(-1) != 1 && t.size(-1) != 1) t = t.contiguous();
+    if (t.dim() > 3) t = t.flatten(0, -2);
+    if (t.dim() == 2) return {t, 1, t.size(0), 0, t.stride(0), t.size(1)};
+    return {t, t.size(0), t.size(1), t.stride(0), t.stride(1), t.size(2)};
+}
+
+// 8-bit checkpoint of a non-empty x
+Tensor checkpoint8(const Tensor& x) {
+    const c10::DeviceGuard guard(x.device());
+    const Rows r = rows_of(x.detach());
+    Tensor saved = bytes(size_of(api.ckpt_bytes(r.n0 * r.n1, r.C), "sad_checkpoint8_bytes"), x);
+    check(api.ckpt_save(r.n0, r.n1, r.C, kind_of(x.scalar_type()), r.t.data_ptr(), r.s0, r.s1, saved.data_ptr(), stream_of(x)),
+          "sad_checkpoint8_save");
+    return saved;
+}
+
+// (dW [N,K], db [N] or undefined), non-empty dy and K > 0
+std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& saved, int64_t K, bool bias) {
+    const c10::DeviceGuard guard(dy.device());
+    const Rows r = rows_of(dy.detach());
+    const int kind = kind_of(dy.scalar_type());
+    Tensor dw = at::empty({r.C, K}, dy.options().dtype(at::kFloat)), db;
+    if (bias) db = at::empty({r.C}, dw.options());
+    const Tensor ws = bytes(size_of(api.wgrad_ws(r.n0 * r.n1, r.C, K, kind), "sad_weight_grad8_workspace_bytes"), dy);
+    check(api.wgrad(r.n0, r.n1, r.C, K, kind, r.t.data_ptr(), r.s0, r.s1, saved.data_ptr(), ptr<float>(dw), ptr<float>(db), ws.data_ptr(),
+                    stream_of(dy)),
+          "sad_weight_grad8");
+    return {dw, db};
+}
+
+// x w^T + b for x [..., K].  A time-major activation seen as [B,T,K] is multiplied as its rows lie in memory, and y comes
+// back in the same order.
+Tensor linear_rows(const Tensor& x, const Tensor& w, const OptTensor& b) {
+    const bool swap = x.dim() == 3 && !x.is_contiguous() && x.transpose(0, 1).is_contiguous();
+    const Tensor xt = swap ? x.transpose(0, 1) : x;
+    auto lead = xt.sizes().vec();
+    const Tensor y = at::linear(xt.reshape({-1, x.size(-1)}), w, b);
+    lead.back() = w.size(0);
+    return swap ? y.view(lead).transpose(0, 1) : y.view(lead);
+}
+
+struct Linear8 : torch::autograd::Function<Linear8> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+        const Tensor w = weight.to(x.scalar_type());
+        OptTensor b;
+        if (bias.has_value()) b = bias->to(x.scalar_type());
+        Tensor y = linear_rows(x, w, b), saved;
+        const bool keep = weight.requires_grad() || (bias.has_value() && bias->requires_grad());
+        if (keep && x.numel() > 0) saved = checkpoint8(x);
+        ctx->save_for_backward({x.requires_grad() ? w : Tensor(), saved});
+        ctx->saved_data["s"] = std::vector<int64_t>{keep, bias.has_value(), weight.size(1), (int64_t)weight.scalar_type(),
+                                                    bias.has_value() ? (int64_t)bias->scalar_type() : 0};
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list gout) {
+        const Tensor& dy = gout[0];
+        const auto saved = ctx->get_saved_variables();
+        const auto v = ctx->saved_data["s"].toIntVector();
+        Tensor dx, dw, db;
+        {
+            at::AutoGradMode no_grad(false);
+            if (ctx->needs_input_grad(0)) dx = linear_rows(dy, saved[0].t(), std::nullopt);
+            if (v[0]) {
+                if (dy.numel() > 0 && saved[1].defined()) std::tie(dw, db) = weight_grad8(dy, saved[1], v[2], v[1] != 0);
+                else {
+                    dw = at::zeros({dy.size(-1), v[2]}, dy.options().dtype(at::kFloat));
+                    if (v[1]) db = at::zeros({dy.size(-1)}, dw.options());
+                }
+                dw = ctx->needs_input_grad(1) ? dw.to((at::ScalarType)v[3]) : Tensor();
+                if (v[1]) db = ctx->needs_input_grad(2) ? db.to((at::ScalarType)v[4]) : Tensor();
+            }
+        }
+        return once({dx, dw, db}, "linear8");
+    }
+};
+
+Tensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.has_value() && bias->requires_grad())))
+        return Linear8::apply(x, weight, bias);
+    OptTensor b;
+    if (bias.has_value()) b = bias->to(x.scalar_type());
+    return linear_rows(x, weight.to(x.scalar_type()), b);
+}
+
+}  // namespace
+
+TORCH_LIBRARY(sad_amd, m) {
+    m.def("bind(int[] addresses) -> ()", &bind);
+    m.def("gated_scan(Tensor z, Tensor? h0, Tensor? lengths, bool reverse, bool gated, bool int8) -> (Tensor, Tensor)", &gated_scan);
+    m.def("linear8(Tensor x, Tensor weight, Tensor? bias) -> Tensor", &linear8);
+}

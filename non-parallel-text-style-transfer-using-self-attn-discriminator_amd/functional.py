@@ -715,13 +715,15 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
-def _like_rows(t, last):
-    """New tensor [.., .., last] of t's type with the order of t's first two axes in memory."""
-    n0, n1, _ = t.shape
-    s0, s1, _ = t.stride()
-    if s0 < s1 and n0 > 1 and n1 > 1:
-        return torch.empty((n1, n0, last), dtype=t.dtype, device=t.device).transpose(0, 1)
-    return torch.empty((n0, n1, last), dtype=t.dtype, device=t.device)
+_op_cache = {}
+
+
+def _op(name):
+    """An autograd node of csrc/torch_ops.cpp."""
+    op = _op_cache.get(name)
+    if op is None:
+        op = _op_cache[name] = getattr(_lib.load_ops(), name).default
+    return op
 
 
 def _scan_parts(width, gated_output):
@@ -750,85 +752,6 @@ def _scan_lengths(lengths, B, T, dev):
     elif lengths.dtype == torch.int64:
         lengths = lengths.clamp(0, T)               # before it is narrowed
     return lengths.to(device=dev, dtype=torch.int32, non_blocking=True).contiguous()
-
-
-_scan_plans = {}
-
-
-def _scan_plan(B, T, D, gated):
-    """Bytes of (workspace, 0 where the library needs none; kept states, padded to 16; codes) of a shape."""
-    key = (B, T, D, gated)
-    plan = _scan_plans.get(key)
-    if plan is None:
-        lib = _lib.load()
-        ws, kept, codes = (lib.sad_gated_scan_workspace_bytes(B, T, D), lib.sad_gated_scan_kept_bytes(B, T, D),
-                           lib.sad_gated_scan_codes_bytes(B, T, D, gated))
-        if ws == 0:
-            raise RuntimeError("libsad sad_gated_scan_workspace_bytes failed: " + _lib.last_error())
-        if len(_scan_plans) > 4096:
-            _scan_plans.clear()
-        plan = _scan_plans[key] = (ws if ws > 16 else 0, (kept + 15) // 16 * 16, codes)
-    return plan
-
-
-def _scan_forward(z, h0, lengths, reverse, gated, int8, track):
-    """(y, h_last, kept states and, behind them, the codes; None without track)."""
-    B, T, W = z.shape
-    D = W // (3 if gated else 2)
-    dev = z.device
-    ws_bytes, kept_bytes, code_bytes = _scan_plan(B, T, D, gated)
-    y = _like_rows(z, D)
-    h_last = torch.empty((B, D), dtype=torch.float32, device=dev)
-    kept = torch.empty(kept_bytes + (code_bytes if int8 else 0), dtype=torch.uint8, device=dev) if track else None
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else h_last      # any address where none is needed
-    kp = kept.data_ptr() if track else None
-    zs, ys = z.stride(), y.stride()
-    a = _lib.SadScanArgs(B, T, D, _KINDS[z.dtype], gated, reverse, z.data_ptr(), zs[0], zs[1], _addr(lengths), _addr(h0),
-                         y.data_ptr(), ys[0], ys[1], h_last.data_ptr(), kp, kp + kept_bytes if track and int8 else None)
-    _launch("sad_gated_scan_fwd", dev, ctypes.byref(a), ws.data_ptr())
-    return y, h_last, kept
-
-
-class _GatedScan(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, h0, lengths, reverse, gated, int8):
-        y, h_last, kept = _scan_forward(z, h0, lengths, reverse, gated, int8, True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(None if int8 else z, lengths, kept)
-        ctx.scan = (z.dtype, z.shape, z.stride(), y.shape, reverse, gated, z.is_contiguous())
-        return y, h_last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dh_last):
-        z, lengths, kept = ctx.saved_tensors
-        dtype, zshape, zstride, yshape, reverse, gated, plain = ctx.scan
-        if dy is None and dh_last is None:
-            return (None,) * 6
-        B, T, D = yshape
-        dev = kept.device
-        if dy is not None:
-            if dy.stride(2) != 1:
-                dy = dy.contiguous()
-            ds = dy.stride()
-        else:
-            ds = (0, 0)
-        if dh_last is not None:
-            dh_last = dh_last.contiguous()
-        if not plain and _is_dense(zshape, zstride):
-            dz = torch.empty_strided(zshape, zstride, dtype=dtype, device=dev)
-        else:
-            dz = torch.empty(zshape, dtype=dtype, device=dev)
-        gs = dz.stride()
-        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
-        ws_bytes, kept_bytes, _ = _scan_plan(B, T, D, gated)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else dz
-        kp = kept.data_ptr()
-        a = _lib.SadScanArgs(B, T, D, _KINDS[dtype], gated, reverse, _addr(z), zstride[0], zstride[1], _addr(lengths), None,
-                             None, 0, 0, None, kp, kp + kept_bytes if z is None else None,
-                             _addr(dy), ds[0], ds[1], _addr(dh_last), dz.data_ptr(), gs[0], gs[1], _addr(dh0))
-        _launch("sad_gated_scan_bwd", dev, ctypes.byref(a), ws.data_ptr())
-        return (dz if ctx.needs_input_grad[0] else None, dh0, None, None, None, None)
 
 
 def gated_scan(z, h0=None, lengths=None, reverse=False, gated_output=True, save="input"):
@@ -867,9 +790,7 @@ def gated_scan(z, h0=None, lengths=None, reverse=False, gated_output=True, save=
         z = z.contiguous()
     if h0 is not None:
         h0 = h0.contiguous()
-    if torch.is_grad_enabled() and (z.requires_grad or (h0 is not None and h0.requires_grad)):
-        return _GatedScan.apply(z, h0, lengths, bool(reverse), bool(gated_output), save == "int8")
-    return _scan_forward(z, h0, lengths, bool(reverse), bool(gated_output), False, False)[:2]
+    return _op("gated_scan")(z, h0, lengths, bool(reverse), bool(gated_output), save == "int8")
 
 
 def _overlaps(a, b):
@@ -1004,44 +925,6 @@ def weight_grad8(dy, ckpt, bias=False):
     return (dw, db) if bias else dw
 
 
-def _linear_rows(x, w, b):
-    """x w^T + b for x [..., K].  A time-major activation seen as [B,T,K] is multiplied as its rows lie in memory, and y
-    comes back in the same order."""
-    swap = x.dim() == 3 and not x.is_contiguous() and x.transpose(0, 1).is_contiguous()
-    y = torch.nn.functional.linear((x.transpose(0, 1) if swap else x).reshape(-1, x.shape[-1]), w, b)
-    if swap:
-        return y.view(x.shape[1], x.shape[0], -1).transpose(0, 1)
-    return y.view(*x.shape[:-1], w.shape[0])
-
-
-class _Linear8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        w = weight.to(x.dtype)
-        y = _linear_rows(x, w, bias.to(x.dtype) if bias is not None else None)
-        ctx.saved8 = saved = None
-        if ctx.needs_input_grad[1] or (bias is not None and ctx.needs_input_grad[2]):
-            ck = checkpoint8(x)
-            saved, ctx.saved8 = ck.saved, (ck.shape, ck.dtype)
-        ctx.save_for_backward(w if ctx.needs_input_grad[0] else None, saved)
-        ctx.linear = (weight.dtype, bias.dtype if bias is not None else None)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        w, saved = ctx.saved_tensors
-        wdtype, bdtype = ctx.linear
-        dx = _linear_rows(dy, w.t(), None) if ctx.needs_input_grad[0] else None
-        dw = db = None
-        if ctx.saved8 is not None:
-            r = weight_grad8(dy, Checkpoint8(saved, *ctx.saved8), bias=bdtype is not None)
-            dw, db = r if bdtype is not None else (r, None)
-            dw = dw.to(wdtype) if ctx.needs_input_grad[1] else None
-            db = db.to(bdtype) if db is not None and ctx.needs_input_grad[2] else None
-        return dx, dw, db
-
-
 def linear8(x, weight, bias=None):
     """``torch.nn.functional.linear`` that keeps its input in 8 bits for the backward pass: y and dx are the linear layer's,
     dW (and db) come from ``weight_grad8``.  ``x`` [..., K] float32 / bfloat16 / float16; ``weight`` [N,K] and ``bias``
@@ -1054,6 +937,4 @@ def linear8(x, weight, bias=None):
         if t is not None and (t.dtype not in (torch.float32, x.dtype) or t.device != x.device or tuple(t.shape) != shape):
             raise RuntimeError("%s must be float32 or %s %s on %s" % (name, x.dtype, shape, x.device))
     _need_device(x, "x")
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        return _Linear8.apply(x, weight, bias)
-    return _linear_rows(x, weight.to(x.dtype), bias.to(x.dtype) if bias is not None else None)
+    return _op("linear8")(x, weight, bias)

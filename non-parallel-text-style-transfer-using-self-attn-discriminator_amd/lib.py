@@ -178,6 +178,28 @@ def load():
     return lib
 
 
+OPS_PATH = os.path.join(_HERE, "_native", "libsad_torch.so")
+_ops = None
+
+
+def load_ops():
+    """torch.ops.sad_amd: the autograd nodes of csrc/torch_ops.cpp, bound to the loaded libsad."""
+    global _ops
+    if _ops is not None:
+        return _ops
+    lib = load()
+    import torch
+    if not os.path.exists(OPS_PATH):
+        raise RuntimeError("libsad_torch.so not found at %s; build it with `bash <package>/csrc/build.sh`." % OPS_PATH)
+    torch.ops.load_library(OPS_PATH)
+    names = ("sad_last_error", "sad_gated_scan_workspace_bytes", "sad_gated_scan_kept_bytes", "sad_gated_scan_codes_bytes",
+             "sad_gated_scan_fwd", "sad_gated_scan_bwd", "sad_checkpoint8_bytes", "sad_checkpoint8_save",
+             "sad_weight_grad8_workspace_bytes", "sad_weight_grad8")
+    torch.ops.sad_amd.bind([ctypes.cast(getattr(lib, n), c_void_p).value for n in names])
+    _ops = torch.ops.sad_amd
+    return _ops
+
+
 def last_error():
     return load().sad_last_error().decode("utf-8", "replace")
 

@@ -575,3 +575,18 @@ def test_saved_input_may_not_change():
     y, _ = Fn.gated_scan(zz, save="int8")       # nothing of z is kept
     zz.add_(1.0)
     y.sum().backward()
+
+
+def test_no_second_derivative():
+    """create_graph works; differentiating the gradient again raises instead of returning something wrong."""
+    torch, _ = _t()
+    from sad_amd import functional as Fn
+    z = torch.randn(2, 20, 3 * 8, device="cuda", requires_grad=True)
+    y, _ = Fn.gated_scan(z)
+    g, = torch.autograd.grad(y.sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        g.sum().backward()
+    w = torch.randn(5, 24, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(Fn.linear8(z, w).sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        g.sum().backward()

@@ -137,6 +137,7 @@ def test_c_entries_refuse_without_a_launch():
     assert l.sad_gated_scan_kept_bytes(2, 33, 5) == 2 * 3 * 5 * 4
     assert l.sad_gated_scan_codes_bytes(2, 33, 33, 1) == 2 * 3 * (3 * (33 + 2) * 16 + 4)
     assert l.sad_checkpoint8_bytes(7, 33) == 7 * 68 and l.sad_checkpoint8_bytes(0, 3) == 0
+    assert l.sad_checkpoint8_bytes(1 << 30, 1) > 0 and l.sad_checkpoint8_bytes((1 << 30) + 1, 1) == 0
     assert l.sad_weight_grad8_workspace_bytes(5, 0, 3, lib.SRC_BF16) == 0
     a = lib.SadScanArgs()
     one = ctypes.c_void_p(16)                                       # never followed: every call below is refused
