@@ -1,8 +1,9 @@
-// Autograd nodes of the gated scan and of linear8 for torch's dispatcher (torch.ops.sad_amd.*).
+// The gated scan and the 8-bit checkpoints for torch's dispatcher (torch.ops.sad_amd.*), with their autograd nodes.
 //
 // functional.py checks the arguments and calls these; they allocate, fill the argument structs and launch through libsad's
-// C-ABI.  They are here and not in Python because the calls are short: the backward pass runs on autograd's device thread,
-// where a Python node first has to take the interpreter lock from the thread that waits for it.
+// C-ABI.  They are here and not in Python because the calls are short: a backward pass runs on autograd's device thread, where
+// a Python node first has to take the interpreter lock from the thread that waits for it (a training call at [64, 23, 512]
+// took 115 us with Python nodes and takes 38).
 //
 // The library's functions are handed in as addresses (sad_amd::bind), so this file does not link libsad and follows whichever
 // build of it the package loaded.
@@ -29,19 +30,21 @@ struct Api {
     decltype(&sad_gated_scan_codes_bytes) scan_codes = nullptr;
     decltype(&sad_gated_scan_fwd) scan_fwd = nullptr;
     decltype(&sad_gated_scan_bwd) scan_bwd = nullptr;
+    decltype(&sad_gated_scan_step) scan_step = nullptr;
     decltype(&sad_checkpoint8_bytes) ckpt_bytes = nullptr;
     decltype(&sad_checkpoint8_save) ckpt_save = nullptr;
+    decltype(&sad_checkpoint8_restore) ckpt_restore = nullptr;
     decltype(&sad_weight_grad8_workspace_bytes) wgrad_ws = nullptr;
     decltype(&sad_weight_grad8) wgrad = nullptr;
 } api;
 
 // addresses in the order of Api's members
 void bind(at::IntArrayRef a) {
-    TORCH_CHECK(a.size() == 10, "expected 10 addresses");
+    TORCH_CHECK(a.size() == 12, "expected 12 addresses");
     int i = 0;
     auto take = [&](auto& f) { f = reinterpret_cast<std::decay_t<decltype(f)>>(a[i++]); };
     take(api.last_error); take(api.scan_ws); take(api.scan_kept); take(api.scan_codes); take(api.scan_fwd); take(api.scan_bwd);
-    take(api.ckpt_bytes); take(api.ckpt_save); take(api.wgrad_ws); take(api.wgrad);
+    take(api.scan_step); take(api.ckpt_bytes); take(api.ckpt_save); take(api.ckpt_restore); take(api.wgrad_ws); take(api.wgrad);
 }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, "libsad ", what, " failed (", rc, "): ", api.last_error()); }
@@ -162,7 +165,20 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& z, const OptTensor& h0, cons
     return {y, h_last};
 }
 
-// ---- linear8 ------------------------------------------------------------------------------------------------------------
+// y; the new states go to h_out (h itself updates in place)
+Tensor gated_scan_step(const Tensor& z, const Tensor& h, const OptTensor& alive, bool gated, const Tensor& h_out) {
+    const c10::DeviceGuard guard(z.device());
+    Tensor y = at::empty({h.size(0), h.size(1)}, z.options());
+    if (h.size(0) == 0) return y;
+    const Tensor zc = z.stride(1) == 1 ? z : z.contiguous(), ac = alive.has_value() ? alive->contiguous() : Tensor();
+    check(api.scan_step((int)h.size(0), (int)h.size(1), kind_of(z.scalar_type()), gated, zc.data_ptr(), zc.stride(0), ptr<float>(h),
+                        h.stride(0), ptr<uint8_t>(ac), y.data_ptr(), y.stride(0), ptr<float>(h_out), h_out.stride(0), stream_of(z)),
+          "sad_gated_scan_step");
+    if (!h_out.is_inference()) h_out.unsafeGetTensorImpl()->bump_version();
+    return y;
+}
+
+// ---- checkpoints, linear8 ------------------------------------------------------------------------------------------------------------
 struct Rows {
     Tensor t;      // holds the memory
     int64_t n0, n1, s0, s1, C;
@@ -176,9 +192,10 @@ Rows rows_of(Tensor t) {
     return {t, t.size(0), t.size(1), t.stride(0), t.stride(1), t.size(2)};
 }
 
-// 8-bit checkpoint of a non-empty x
+// 8-bit checkpoint of x [..., C]
 Tensor checkpoint8(const Tensor& x) {
     const c10::DeviceGuard guard(x.device());
+    if (x.numel() == 0) return bytes(0, x);
     const Rows r = rows_of(x.detach());
     Tensor saved = bytes(size_of(api.ckpt_bytes(r.n0 * r.n1, r.C), "sad_checkpoint8_bytes"), x);
     check(api.ckpt_save(r.n0, r.n1, r.C, kind_of(x.scalar_type()), r.t.data_ptr(), r.s0, r.s1, saved.data_ptr(), stream_of(x)),
@@ -186,15 +203,30 @@ Tensor checkpoint8(const Tensor& x) {
     return saved;
 }
 
-// (dW [N,K], db [N] or undefined), non-empty dy and K > 0
+// the values a checkpoint stands for, contiguous
+Tensor restore8(const Tensor& saved, at::IntArrayRef size, at::ScalarType dtype) {
+    const c10::DeviceGuard guard(saved.device());
+    Tensor out = at::empty(size, saved.options().dtype(dtype));
+    if (out.numel() == 0) return out;
+    check(api.ckpt_restore(out.numel() / size.back(), size.back(), kind_of(dtype), saved.data_ptr(), out.data_ptr(), stream_of(saved)),
+          "sad_checkpoint8_restore");
+    return out;
+}
+
+// (dW [N,K], db [N] or an empty tensor)
 std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& saved, int64_t K, bool bias) {
     const c10::DeviceGuard guard(dy.device());
+    if (dy.numel() == 0 || K == 0) {
+        const auto options = dy.options().dtype(at::kFloat);
+        const Tensor dw = at::zeros({dy.size(-1), K}, options);
+        if (!bias) return {dw, at::empty({0}, options)};
+        return {dw, dy.numel() == 0 ? at::zeros({dy.size(-1)}, options) : dy.detach().to(at::kFloat).reshape({-1, dy.size(-1)}).sum(0)};
+    }
     const Rows r = rows_of(dy.detach());
     const int kind = kind_of(dy.scalar_type());
-    Tensor dw = at::empty({r.C, K}, dy.options().dtype(at::kFloat)), db;
-    if (bias) db = at::empty({r.C}, dw.options());
+    Tensor dw = at::empty({r.C, K}, dy.options().dtype(at::kFloat)), db = at::empty({bias ? r.C : 0}, dw.options());
     const Tensor ws = bytes(size_of(api.wgrad_ws(r.n0 * r.n1, r.C, K, kind), "sad_weight_grad8_workspace_bytes"), dy);
-    check(api.wgrad(r.n0, r.n1, r.C, K, kind, r.t.data_ptr(), r.s0, r.s1, saved.data_ptr(), ptr<float>(dw), ptr<float>(db), ws.data_ptr(),
+    check(api.wgrad(r.n0, r.n1, r.C, K, kind, r.t.data_ptr(), r.s0, r.s1, saved.data_ptr(), ptr<float>(dw), bias ? ptr<float>(db) : nullptr, ws.data_ptr(),
                     stream_of(dy)),
           "sad_weight_grad8");
     return {dw, db};
@@ -218,7 +250,7 @@ struct Linear8 : torch::autograd::Function<Linear8> {
         if (bias.has_value()) b = bias->to(x.scalar_type());
         Tensor y = linear_rows(x, w, b), saved;
         const bool keep = weight.requires_grad() || (bias.has_value() && bias->requires_grad());
-        if (keep && x.numel() > 0) saved = checkpoint8(x);
+        if (keep) saved = checkpoint8(x);
         ctx->save_for_backward({x.requires_grad() ? w : Tensor(), saved});
         ctx->saved_data["s"] = std::vector<int64_t>{keep, bias.has_value(), weight.size(1), (int64_t)weight.scalar_type(),
                                                     bias.has_value() ? (int64_t)bias->scalar_type() : 0};
@@ -233,13 +265,9 @@ struct Linear8 : torch::autograd::Function<Linear8> {
             at::AutoGradMode no_grad(false);
             if (ctx->needs_input_grad(0)) dx = linear_rows(dy, saved[0].t(), std::nullopt);
             if (v[0]) {
-                if (dy.numel() > 0 && saved[1].defined()) std::tie(dw, db) = weight_grad8(dy, saved[1], v[2], v[1] != 0);
-                else {
-                    dw = at::zeros({dy.size(-1), v[2]}, dy.options().dtype(at::kFloat));
-                    if (v[1]) db = at::zeros({dy.size(-1)}, dw.options());
-                }
+                std::tie(dw, db) = weight_grad8(dy, saved[1], v[2], v[1] != 0);
                 dw = ctx->needs_input_grad(1) ? dw.to((at::ScalarType)v[3]) : Tensor();
-                if (v[1]) db = ctx->needs_input_grad(2) ? db.to((at::ScalarType)v[4]) : Tensor();
+                db = v[1] && ctx->needs_input_grad(2) ? db.to((at::ScalarType)v[4]) : Tensor();
             }
         }
         return once({dx, dw, db}, "linear8");
@@ -259,5 +287,9 @@ Tensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
 TORCH_LIBRARY(sad_amd, m) {
     m.def("bind(int[] addresses) -> ()", &bind);
     m.def("gated_scan(Tensor z, Tensor? h0, Tensor? lengths, bool reverse, bool gated, bool int8) -> (Tensor, Tensor)", &gated_scan);
+    m.def("gated_scan_step(Tensor z, Tensor h, Tensor? alive, bool gated, Tensor(a!) h_out) -> Tensor", &gated_scan_step);
+    m.def("checkpoint8(Tensor x) -> Tensor", &checkpoint8);
+    m.def("restore8(Tensor saved, int[] size, ScalarType dtype) -> Tensor", &restore8);
+    m.def("weight_grad8(Tensor dy, Tensor saved, int K, bool bias) -> (Tensor, Tensor)", &weight_grad8);
     m.def("linear8(Tensor x, Tensor weight, Tensor? bias) -> Tensor", &linear8);
 }

@@ -678,48 +678,11 @@ def _need_device(t, what):
         raise RuntimeError("%s must be on the HIP device (got a CPU tensor); there is no CPU path" % what)
 
 
-# Sizes the library names, by (function, arguments): a call costs more host time than the lookup.
-_sizes = {}
-
-
-def _bytes(dev, name, *args):
-    """Uninitialised device memory of the size that the library's function `name` gives for `args` (0 = it refused)."""
-    n = _sizes.get((name, args))
-    if n is None:
-        n = getattr(_lib.load(), name)(*args)
-        if n == 0:
-            raise RuntimeError("libsad %s failed: %s" % (name, _lib.last_error()))
-        if len(_sizes) > 4096:
-            _sizes.clear()
-        _sizes[(name, args)] = n
-    return torch.empty(n, dtype=torch.uint8, device=dev)
-
-
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-
-
-def _launch(name, dev, *args):
-    """Library entry `name` with `args` and the current stream of `dev`."""
-    fn = getattr(_lib.load(), name)
-    cur = _current_device()
-    if dev.index is None or dev.index == cur:
-        rc = fn(*args, _RAW_STREAM(cur))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _RAW_STREAM(dev.index))
-    if rc != 0:
-        _lib.check(rc, name)
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
 _op_cache = {}
 
 
 def _op(name):
-    """An autograd node of csrc/torch_ops.cpp."""
+    """An operator of csrc/torch_ops.cpp."""
     op = _op_cache.get(name)
     if op is None:
         op = _op_cache[name] = getattr(_lib.load_ops(), name).default
@@ -811,7 +774,7 @@ def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
     ``z`` [B,3D] / [B,2D] are the token's pre-activations, ``h`` [B,D] float32 the states.  The new states go to ``h_out``
     (a new tensor if None; ``h`` itself updates in place).  ``alive`` [B] bool: a sentence that has ended keeps its state
     and gives y = 0.  No gradient (train with ``gated_scan``)."""
-    kind = _kind(z, "z")
+    _kind(z, "z")
     if z.dim() != 2:
         raise RuntimeError("z must be [B,3D] or [B,2D], got %s" % (tuple(z.shape),))
     D = _scan_parts(z.shape[1], gated_output)
@@ -833,34 +796,12 @@ def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
         if B and _overlaps(h_out, z):
             raise RuntimeError("h_out must not overlap z")
     _need_device(z, "z")
-    y = torch.empty((B, D), dtype=z.dtype, device=dev)
-    if B == 0:
-        return y, h_out
-    if z.stride(1) != 1:
-        z = z.contiguous()
-    if alive is not None:
-        alive = alive.contiguous()
-    _launch("sad_gated_scan_step", dev, B, D, kind, int(gated_output), z.data_ptr(), z.stride(0), h.data_ptr(), h.stride(0), _addr(alive),
-            y.data_ptr(), D, h_out.data_ptr(), h_out.stride(0))
-    return y, h_out
+    return _op("gated_scan_step")(z, h, alive, bool(gated_output), h_out), h_out
 
 
 # ------------------------------------------------------------------------------------------------
 # 8-bit activation checkpoints (include/sad.h, sad_checkpoint8_*, sad_weight_grad8)
 # ------------------------------------------------------------------------------------------------
-def _rows2(t):
-    """(t, n0, n1, stride0, stride1): the rows of t [..., C] in their order, without a copy where two strides say it."""
-    if t.dim() == 1:
-        t = t.unsqueeze(0)
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
-        t = t.contiguous()
-    if t.dim() > 3:
-        t = t.flatten(0, -2)
-    if t.dim() == 2:
-        return t, 1, t.shape[0], 0, t.stride(0)
-    return t, t.shape[0], t.shape[1], t.stride(0), t.stride(1)
-
-
 class Checkpoint8:
     """A tensor [..., C] kept in 8 bits (``checkpoint8``): ``saved`` (uint8: codes, then exponents), ``shape``, ``dtype``."""
 
@@ -869,12 +810,7 @@ class Checkpoint8:
 
     def restore(self):
         """The values the codes stand for, as a new contiguous tensor of the original type."""
-        out = torch.empty(self.shape, dtype=self.dtype, device=self.saved.device)
-        if out.numel():
-            C = self.shape[-1]
-            _launch("sad_checkpoint8_restore", out.device, out.numel() // C, C, _KINDS[self.dtype], self.saved.data_ptr(),
-                    out.data_ptr())
-        return out
+        return _op("restore8")(self.saved, self.shape, self.dtype)
 
 
 def checkpoint8(x):
@@ -882,26 +818,18 @@ def checkpoint8(x):
     channels, the smallest whose 127 steps reach the largest finite entry.  An entry comes back within half a step (at most
     1/127 of that largest entry; 1/63 where the type's own largest values leave no room above); infinities and NaN come
     back as NaN and leave their neighbours alone.  Returns a ``Checkpoint8``; no gradient flows through it."""
-    kind = _kind(x, "x")
+    _kind(x, "x")
     if x.dim() == 0:
         raise RuntimeError("x must have a channel axis")
     _need_device(x, "x")
-    shape, dev = x.shape, x.device
-    x = x.detach()
-    if x.numel() == 0:
-        return Checkpoint8(torch.empty(0, dtype=torch.uint8, device=dev), shape, x.dtype)
-    x, n0, n1, s0, s1 = _rows2(x)
-    C = shape[-1]
-    saved = _bytes(dev, "sad_checkpoint8_bytes", n0 * n1, C)
-    _launch("sad_checkpoint8_save", dev, n0, n1, C, kind, x.data_ptr(), s0, s1, saved.data_ptr())
-    return Checkpoint8(saved, shape, x.dtype)
+    return Checkpoint8(_op("checkpoint8")(x), x.shape, x.dtype)
 
 
 def weight_grad8(dy, ckpt, bias=False):
     """Weight gradient ``dW [N,K] = dy^T x^`` (float32) of a linear layer from the checkpoint of its input ``x`` [..., K];
     ``dy`` [..., N] has x's leading shape and type.  ``bias=True`` adds ``db [N] = sum dy``: ``(dW, db)``.  Sums are
     float32 in a fixed order: the same call gives the same bits."""
-    kind = _kind(dy, "dy")
+    _kind(dy, "dy")
     if dy.dtype != ckpt.dtype or dy.dim() != len(ckpt.shape) or dy.shape[:-1] != ckpt.shape[:-1]:
         raise RuntimeError("dy %s %s does not belong to a checkpoint of %s %s"
                            % (dy.dtype, tuple(dy.shape), ckpt.dtype, tuple(ckpt.shape)))
@@ -909,19 +837,7 @@ def weight_grad8(dy, ckpt, bias=False):
     if ckpt.saved.device != dev:
         raise RuntimeError("dy is on %s, the checkpoint on %s" % (dev, ckpt.saved.device))
     _need_device(dy, "dy")
-    N, K = dy.shape[-1], ckpt.shape[-1]
-    dy = dy.detach()
-    if dy.numel() == 0 or K == 0:
-        dw = torch.zeros((N, K), dtype=torch.float32, device=dev)
-        if not bias:
-            return dw
-        return dw, (torch.zeros(N, dtype=torch.float32, device=dev) if dy.numel() == 0 else dy.float().flatten(0, -2).sum(0))
-    dy, n0, n1, s0, s1 = _rows2(dy)
-    dw = torch.empty((N, K), dtype=torch.float32, device=dev)
-    db = torch.empty(N, dtype=torch.float32, device=dev) if bias else None
-    ws = _bytes(dev, "sad_weight_grad8_workspace_bytes", n0 * n1, N, K, kind)
-    _launch("sad_weight_grad8", dev, n0, n1, N, K, kind, dy.data_ptr(), s0, s1, ckpt.saved.data_ptr(), dw.data_ptr(), _addr(db),
-            ws.data_ptr())
+    dw, db = _op("weight_grad8")(dy, ckpt.saved, ckpt.shape[-1], bool(bias))
     return (dw, db) if bias else dw
 
 

@@ -193,8 +193,8 @@ def load_ops():
         raise RuntimeError("libsad_torch.so not found at %s; build it with `bash <package>/csrc/build.sh`." % OPS_PATH)
     torch.ops.load_library(OPS_PATH)
     names = ("sad_last_error", "sad_gated_scan_workspace_bytes", "sad_gated_scan_kept_bytes", "sad_gated_scan_codes_bytes",
-             "sad_gated_scan_fwd", "sad_gated_scan_bwd", "sad_checkpoint8_bytes", "sad_checkpoint8_save",
-             "sad_weight_grad8_workspace_bytes", "sad_weight_grad8")
+             "sad_gated_scan_fwd", "sad_gated_scan_bwd", "sad_gated_scan_step", "sad_checkpoint8_bytes", "sad_checkpoint8_save",
+             "sad_checkpoint8_restore", "sad_weight_grad8_workspace_bytes", "sad_weight_grad8")
     torch.ops.sad_amd.bind([ctypes.cast(getattr(lib, n), c_void_p).value for n in names])
     _ops = torch.ops.sad_amd
     return _ops
