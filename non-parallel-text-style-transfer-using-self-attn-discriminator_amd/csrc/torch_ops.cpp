@@ -66,6 +66,12 @@ variable_list once(variable_list grads, const char* name) {
     return (*fn)(std::move(grads));
 }
 
+// sizes go into 32-bit fields
+int dim32(int64_t n) {
+    TORCH_CHECK(n <= INT32_MAX, "a size of ", n, " is beyond the supported maximum");
+    return (int)n;
+}
+
 // ---- gated scan -------------------------------------------------------------------------------------------------------
 struct ScanShape {
     int64_t B, T, D, ws, kept, codes;
@@ -73,9 +79,10 @@ struct ScanShape {
 ScanShape scan_shape(const Tensor& z, bool gated) {
     ScanShape s;
     s.B = z.size(0); s.T = z.size(1); s.D = z.size(2) / (gated ? 3 : 2);
-    s.ws = (int64_t)size_of(api.scan_ws((int)s.B, (int)s.T, (int)s.D), "sad_gated_scan_workspace_bytes");
-    s.kept = ((int64_t)api.scan_kept((int)s.B, (int)s.T, (int)s.D) + 15) / 16 * 16;
-    s.codes = (int64_t)api.scan_codes((int)s.B, (int)s.T, (int)s.D, gated);
+    const int B = dim32(s.B), T = dim32(s.T), D = dim32(s.D);
+    s.ws = (int64_t)size_of(api.scan_ws(B, T, D), "sad_gated_scan_workspace_bytes");
+    s.kept = ((int64_t)api.scan_kept(B, T, D) + 15) / 16 * 16;
+    s.codes = (int64_t)api.scan_codes(B, T, D, gated);
     return s;
 }
 
@@ -171,7 +178,7 @@ Tensor gated_scan_step(const Tensor& z, const Tensor& h, const OptTensor& alive,
     Tensor y = at::empty({h.size(0), h.size(1)}, z.options());
     if (h.size(0) == 0) return y;
     const Tensor zc = z.stride(1) == 1 ? z : z.contiguous(), ac = alive.has_value() ? alive->contiguous() : Tensor();
-    check(api.scan_step((int)h.size(0), (int)h.size(1), kind_of(z.scalar_type()), gated, zc.data_ptr(), zc.stride(0), ptr<float>(h),
+    check(api.scan_step(dim32(h.size(0)), dim32(h.size(1)), kind_of(z.scalar_type()), gated, zc.data_ptr(), zc.stride(0), ptr<float>(h),
                         h.stride(0), ptr<uint8_t>(ac), y.data_ptr(), y.stride(0), ptr<float>(h_out), h_out.stride(0), stream_of(z)),
           "sad_gated_scan_step");
     if (!h_out.is_inference()) h_out.unsafeGetTensorImpl()->bump_version();
