@@ -54,7 +54,10 @@ size_t size_of(size_t n, const char* what) {
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
-int kind_of(at::ScalarType t) { return t == at::kFloat ? SAD_SRC_F32 : (t == at::kBFloat16 ? SAD_SRC_BF16 : SAD_SRC_F16); }
+int kind_of(at::ScalarType t) {
+    TORCH_CHECK(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "expected float32, bfloat16 or float16, got ", t);
+    return t == at::kFloat ? SAD_SRC_F32 : (t == at::kBFloat16 ? SAD_SRC_BF16 : SAD_SRC_F16);
+}
 template <class T> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 
 // autograd.Function's once_differentiable: with create_graph the results raise when they are differentiated again
@@ -242,6 +245,7 @@ std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& saved, i
 // x w^T + b for x [..., K].  A time-major activation seen as [B,T,K] is multiplied as its rows lie in memory, and y comes
 // back in the same order.
 Tensor linear_rows(const Tensor& x, const Tensor& w, const OptTensor& b) {
+    const c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::autocast_dispatch_keyset);      // x's type is the caller's choice
     const bool swap = x.dim() == 3 && !x.is_contiguous() && x.transpose(0, 1).is_contiguous();
     const Tensor xt = swap ? x.transpose(0, 1) : x;
     auto lead = xt.sizes().vec();

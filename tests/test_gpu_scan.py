@@ -281,9 +281,9 @@ def test_step_matches_oracle(dtype, B, D):
         _check(_np(y), ref["y"][:, 0], tol + (F + 8) * U * X, _half(DT[dtype]), "y")
         dead = ~alive
         assert torch.equal(out[dead], h[dead]) and (y[dead] == 0).all()
-        kept = h.clone()
+        kept, version = h.clone(), h._version
         y2, same = Fn.gated_scan_step(z, h, alive=alive, gated_output=gated, h_out=h)       # in place
-        assert same is h and torch.equal(h, out) and torch.equal(y2, y) and not torch.equal(kept, h) or dead.all()
+        assert same is h and h._version > version and torch.equal(h, out) and torch.equal(y2, y) and not torch.equal(kept, h) or dead.all()
 
 
 def test_empty_sizes():
@@ -431,6 +431,8 @@ def test_linear8(dtype, bias):
     with torch.no_grad():
         plain = Fn.linear8(x, w, b)
     assert not plain.requires_grad and torch.equal(plain, y) and plain.stride() == y.stride()
+    with torch.autocast("cuda", dtype=torch.float16):                  # the type of x decides, inside autocast too
+        assert torch.equal(Fn.linear8(x, w, b), y)
     one = Fn.linear8(xf[0, 0], wd)
     g1, = torch.autograd.grad(one, wd, dy[0, 0])
     assert tuple(one.shape) == (N,) and g1.abs().max() > 0
