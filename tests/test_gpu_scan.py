@@ -592,3 +592,55 @@ def test_no_second_derivative():
     g, = torch.autograd.grad(Fn.linear8(z, w).sum(), w, create_graph=True)
     with pytest.raises(RuntimeError, match="no second derivative"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("M,N,K", [(903, 4093, 3001), (705, 5101, 4001), (1503, 4001, 2001), (1311, 1501, 300), (2050, 128, 128)],
+                         ids=["256x256", "192x256", "128x320", "128x128", "split"])
+def test_weight_grad_tiles(dtype, M, N, K):
+    """Every output tile of the kernel, at odd sizes with several stages, against a 64-bit product; then with lost entries in
+    the first, a middle and the last stage: their columns are NaN, every other entry keeps its bits."""
+    torch, DT = _t()
+    from sad_amd import functional as Fn
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = torch.randn(M, K, device="cuda", generator=g).to(DT[dtype])
+    dy = torch.randn(M, N, device="cuda", generator=g).to(DT[dtype])
+    ck = Fn.checkpoint8(x)
+    dw, db = Fn.weight_grad8(dy, ck, bias=True)
+    xv, dv = ck.restore().double(), dy.double()
+    assert ((dw.double() - dv.t() @ xv).abs() <= M * U * (dv.abs().t() @ xv.abs())).all()
+    assert ((db.double() - dv.sum(0)).abs() <= M * U * dv.abs().sum(0)).all()
+    bad = x.clone()
+    cols = [0, K // 2, K - 1]
+    for row, col in zip((5, M // 2, M - 1), cols):
+        bad[row, col] = float("inf")
+    dn = Fn.weight_grad8(dy, Fn.checkpoint8(bad))
+    assert torch.isnan(dn[:, cols]).all()
+    rest = [c for c in range(K) if c // 32 not in [c // 32 for c in cols]]
+    assert torch.equal(dn[:, rest], dw[:, rest])
+    assert torch.isfinite(dn).sum() == N * (K - 3)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_int8_lost_entries_in_long_sentences(reverse):
+    """A lost forget gate in the middle of sentences cut along time: its own channel's gradient is NaN on the side the
+    gradient flows to, every other channel keeps its bits."""
+    torch, _ = _t()
+    from sad_amd import functional as Fn
+    torch.manual_seed(4)
+    D = 96
+    z = torch.randn(2, 1500, 3 * D)
+    grads = []
+    for lost in (False, True):
+        zz = z.clone()
+        if lost:
+            zz[1, 700, D + 37] = float("nan")
+        zt = zz.cuda().requires_grad_(True)
+        y, last = Fn.gated_scan(zt, lengths=torch.tensor([1500, 1400]), reverse=reverse, save="int8")
+        y = torch.where(torch.isnan(y), torch.zeros_like(y), y)
+        grads.append(torch.autograd.grad(y.sum(), zt)[0].view(2, 1500, 3, D))
+    other = [c for c in range(D) if c // 32 != 37 // 32]
+    assert torch.equal(grads[0][..., other], grads[1][..., other]) and torch.equal(grads[0][0], grads[1][0])
+    assert torch.isnan(grads[1][1, 700, :2, 37]).all()
+    same_block = [c for c in range(32, 64) if c != 37]
+    assert torch.isfinite(grads[1][..., same_block]).all()

@@ -168,3 +168,18 @@ def test_c_entries_refuse_without_a_launch():
     refused(l.sad_checkpoint8_restore(2, 3, lib.SRC_F32, None, one, None), "saved is NULL")
     refused(l.sad_weight_grad8(1, 2, 3, 4, 9, one, 0, 3, one, one, None, one, None), "kind must be")
     refused(l.sad_weight_grad8(1, 2, 3, 4, lib.SRC_F32, one, 0, 3, one, None, None, one, None), "dw is NULL")
+
+
+def test_missing_operator_library_fails_loudly(monkeypatch):
+    monkeypatch.setattr(lib, "_ops", None)
+    monkeypatch.setattr(lib, "OPS_PATH", "/nonexistent/libsad_torch.so")
+    with pytest.raises(RuntimeError, match="libsad_torch.so not found"):
+        lib.load_ops()
+
+
+def test_operators_are_registered():
+    ops = lib.load_ops()
+    for name in ("gated_scan", "gated_scan_step", "checkpoint8", "restore8", "weight_grad8", "linear8"):
+        assert getattr(ops, name).default is not None
+    with pytest.raises(RuntimeError, match="12 addresses"):
+        ops.bind([0])
