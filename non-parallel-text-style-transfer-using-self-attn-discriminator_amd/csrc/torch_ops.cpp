@@ -213,18 +213,34 @@ Tensor checkpoint8(const Tensor& x) {
     return saved;
 }
 
+// `saved` is the caller's to move, copy and slice: it has to be a whole checkpoint of rows x C entries, on the device
+void need_saved(const Tensor& saved, int64_t rows, int64_t C) {
+    TORCH_CHECK(saved.scalar_type() == at::kByte && saved.is_contiguous(), "a checkpoint's codes are contiguous uint8, got ", saved.scalar_type(),
+                saved.is_contiguous() ? "" : " (not contiguous)");
+    const size_t n = rows > 0 && C > 0 ? size_of(api.ckpt_bytes(rows, C), "sad_checkpoint8_bytes") : 0;
+    TORCH_CHECK((size_t)saved.numel() == n, "a checkpoint of ", rows, " x ", C, " entries holds ", n, " bytes, got ", saved.numel());
+    TORCH_CHECK(saved.is_cuda(), "a checkpoint's codes must be on the HIP device, got ", saved.device(), "; there is no CPU path");
+}
+
 // the values a checkpoint stands for, contiguous
 Tensor restore8(const Tensor& saved, at::IntArrayRef size, at::ScalarType dtype) {
+    TORCH_CHECK(!size.empty(), "a checkpoint has a channel axis");
+    const int64_t n = c10::multiply_integers(size), rows = n > 0 ? n / size.back() : 0;
+    need_saved(saved, rows, size.back());
     const c10::DeviceGuard guard(saved.device());
     Tensor out = at::empty(size, saved.options().dtype(dtype));
-    if (out.numel() == 0) return out;
-    check(api.ckpt_restore(out.numel() / size.back(), size.back(), kind_of(dtype), saved.data_ptr(), out.data_ptr(), stream_of(saved)),
+    if (n == 0) return out;
+    check(api.ckpt_restore(rows, size.back(), kind_of(dtype), saved.data_ptr(), out.data_ptr(), stream_of(saved)),
           "sad_checkpoint8_restore");
     return out;
 }
 
 // (dW [N,K], db [N] or an empty tensor)
 std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& saved, int64_t K, bool bias) {
+    TORCH_CHECK(dy.dim() > 0, "dy must have a channel axis");
+    const int64_t rows = c10::multiply_integers(dy.sizes().slice(0, dy.dim() - 1));
+    need_saved(saved, rows, K);
+    TORCH_CHECK(saved.device() == dy.device(), "dy is on ", dy.device(), ", the checkpoint on ", saved.device());
     const c10::DeviceGuard guard(dy.device());
     if (dy.numel() == 0 || K == 0) {
         const auto options = dy.options().dtype(at::kFloat);

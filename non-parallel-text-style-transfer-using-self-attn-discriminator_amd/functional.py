@@ -803,7 +803,8 @@ def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
 # 8-bit activation checkpoints (include/sad.h, sad_checkpoint8_*, sad_weight_grad8)
 # ------------------------------------------------------------------------------------------------
 class Checkpoint8:
-    """A tensor [..., C] kept in 8 bits (``checkpoint8``): ``saved`` (uint8: codes, then exponents), ``shape``, ``dtype``."""
+    """A tensor [..., C] kept in 8 bits (``checkpoint8``): ``saved`` (uint8: codes, then exponents), ``shape``, ``dtype``.
+    ``saved`` may be moved (to the host and back): it is read where it is whole and on the device, and refused otherwise."""
 
     def __init__(self, saved, shape, dtype):
         self.saved, self.shape, self.dtype = saved, torch.Size(shape), dtype

@@ -1,0 +1,41 @@
+"""CPU checks of what the gated scan's and the 8-bit checkpoints' entry points do with calls a user can make beside the plain
+ones.  Refused calls raise before anything is launched, through functional and through torch.ops.sad_amd alike."""
+import pytest
+import torch
+
+from sad_amd import functional as Fn
+from sad_amd import lib
+
+F32 = torch.float32
+
+
+def _codes(n, **kw):
+    return torch.zeros(n, dtype=torch.uint8, **kw)
+
+
+@pytest.mark.parametrize("saved,shape,message", [
+    (_codes(7 * 68), (7, 33), "must be on the HIP device"),                    # moved to the host
+    (_codes(64), (1000, 33), "holds 68000 bytes, got 64"),                     # a slice of the codes
+    (_codes(7 * 68 + 1), (7, 33), "holds 476 bytes"),
+    (_codes(0), (7, 33), "holds 476 bytes"),
+    (_codes(5), (0, 33), "holds 0 bytes"),
+    (torch.zeros(7 * 68), (7, 33), "contiguous uint8"),
+    (_codes(2 * 7 * 68)[::2], (7, 33), "contiguous uint8"),
+    (_codes(34), (), "channel axis"),
+])
+def test_restore_takes_whole_checkpoints_on_the_device_only(saved, shape, message):
+    with pytest.raises(RuntimeError, match=message):
+        Fn.Checkpoint8(saved, shape, F32).restore()
+
+
+@pytest.mark.parametrize("saved,message", [
+    (_codes(4 * 34), "must be on the HIP device"),
+    (_codes(4 * 34 - 1), "holds 136 bytes, got 135"),
+    (_codes(4 * 34).view(torch.int8), "contiguous uint8"),
+    (_codes(2 * 4 * 34)[::2], "contiguous uint8"),
+])
+def test_weight_gradient_takes_whole_checkpoints_on_the_device_only(saved, message):
+    with pytest.raises(RuntimeError, match=message):
+        lib.load_ops().weight_grad8(torch.zeros(4, 5), saved, 6, True)
+    with pytest.raises(RuntimeError):
+        Fn.weight_grad8(torch.zeros(4, 5), Fn.Checkpoint8(saved, (4, 6), F32), bias=True)
