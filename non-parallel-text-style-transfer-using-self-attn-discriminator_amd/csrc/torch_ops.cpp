@@ -130,19 +130,30 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({int8 ? Tensor() : z, l, kept});
         ctx->saved_data["s"] = std::vector<int64_t>{z.size(0), z.size(1), z.size(2), z.stride(0), z.stride(1), z.stride(2),
-                                                    (int64_t)z.scalar_type(), reverse, gated, h0.has_value()};
+                                                    (int64_t)z.scalar_type(), reverse, gated, h0.has_value(), kept.numel()};
         return {y, h_last};
     }
     static variable_list backward(AutogradContext* ctx, variable_list gout) {
         Tensor dy = gout[0], dh = gout[1];
         if (!dy.defined() && !dh.defined()) return variable_list(6);
         const auto saved = ctx->get_saved_variables();
-        const Tensor &z = saved[0], &lengths = saved[1], &kept = saved[2];
         const auto v = ctx->saved_data["s"].toIntVector();
         const bool reverse = v[7] != 0, gated = v[8] != 0;
+        const at::IntArrayRef size(v.data(), 3), stride(v.data() + 3, 3);
+        // Saved tensors pass through the hooks of the program (save_on_cpu), which keep values and not layouts: what comes
+        // back is read by its own strides.
+        Tensor z = saved[0], lengths = saved[1], kept = saved[2];
+        if (z.defined() && z.stride(2) != 1) z = z.contiguous();
+        if (lengths.defined()) lengths = lengths.contiguous();
+        kept = kept.contiguous();
+        if ((size_t)kept.data_ptr() % 16) kept = kept.clone();
+        TORCH_CHECK(!z.defined() || (z.sizes() == size && z.scalar_type() == (at::ScalarType)v[6] && z.device() == kept.device()),
+                    "gated_scan: the saved z came back as another tensor");
+        TORCH_CHECK(kept.is_cuda() && kept.scalar_type() == at::kByte && kept.numel() == v[10], "gated_scan: the kept states came back as another tensor");
+        TORCH_CHECK(!lengths.defined() || (lengths.scalar_type() == at::kInt && lengths.numel() == size[0] && lengths.device() == kept.device()),
+                    "gated_scan: the lengths came back as another tensor");
         const c10::DeviceGuard guard(kept.device());
         const auto options = kept.options().dtype((at::ScalarType)v[6]);
-        const at::IntArrayRef size(v.data(), 3), stride(v.data() + 3, 3);
         Tensor dz = is_dense(size, stride) ? at::empty_strided(size, stride, options) : at::empty(size, options), dh0;
         const ScanShape s = scan_shape(dz, gated);
         if (dy.defined() && dy.stride(2) != 1) dy = dy.contiguous();
@@ -154,7 +165,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
         a.kind = kind_of(dz.scalar_type()); a.gated = gated; a.reverse = reverse;
         a.lengths = ptr<int32_t>(lengths);
         a.kept = ptr<float>(kept);
-        if (z.defined()) { a.z = z.data_ptr(); a.z_stride_b = stride[0]; a.z_stride_t = stride[1]; }
+        if (z.defined()) { a.z = z.data_ptr(); a.z_stride_b = z.stride(0); a.z_stride_t = z.stride(1); }
         else a.codes = ptr<char>(kept) + s.kept;
         if (dy.defined()) { a.dy = dy.data_ptr(); a.dy_stride_b = dy.stride(0); a.dy_stride_t = dy.stride(1); }
         a.dh_last = ptr<float>(dh);

@@ -32,3 +32,50 @@ def test_checkpoint_moved_to_the_host_and_back():
     shifted = torch.cat([ck.saved[:1], ck.saved])[1:]
     with pytest.raises(RuntimeError, match="16-byte aligned"):
         Fn.Checkpoint8(shifted, ck.shape, ck.dtype).restore()
+
+
+@pytest.mark.parametrize("save", ["input", "int8"])
+@pytest.mark.parametrize("layout", ["time", "wide"])
+def test_saved_tensors_kept_on_the_host(layout, save):
+    """Hooks for saved tensors give z back in another layout than the forward pass saw (save_on_cpu: contiguous)."""
+    torch, Fn = _t()
+    torch.manual_seed(3)
+    B, T, D = 5, 37, 40
+    z = torch.randn(B, T, 3 * D, device="cuda")
+    if layout == "time":
+        z = z.transpose(0, 1).contiguous().transpose(0, 1)
+    else:
+        z = torch.cat([z, z], -1)[..., 7:7 + 3 * D]
+    z.requires_grad_(True)
+    lengths = torch.tensor([37, 0, 12, 36, 1], dtype=torch.int32, device="cuda")
+    dy = torch.randn(B, T, D, device="cuda")
+
+    def grad():
+        y, last = Fn.gated_scan(z, lengths=lengths, save=save)
+        return torch.autograd.grad([y, last], z, [dy, torch.ones_like(last)])[0]
+
+    want = grad()
+    with torch.autograd.graph.save_on_cpu():
+        got = grad()
+    assert torch.equal(got, want)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.transpose(0, -1).contiguous().transpose(0, -1)):
+        got = grad()                                                   # channel stride B, codes not contiguous
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("unpack,message", [
+    (lambda t: t[:1] if t.dim() == 3 else t, "saved z came back"),
+    (lambda t: t.double() if t.dim() == 3 else t, "saved z came back"),
+    (lambda t: t.cpu() if t.dim() == 3 else t, "saved z came back"),
+    (lambda t: t[:-16] if t.element_size() == 1 else t, "kept states came back"),
+    (lambda t: t.cpu() if t.element_size() == 1 else t, "came back"),
+    (lambda t: t.cpu() if t.dtype.itemsize == 4 and t.dim() == 1 else t, "lengths came back"),
+    (lambda t: t.long() if t.dtype.itemsize == 4 and t.dim() == 1 else t, "lengths came back"),
+])
+def test_saved_tensors_that_come_back_as_others_are_refused(unpack, message):
+    torch, Fn = _t()
+    z = torch.randn(2, 20, 3 * 8, device="cuda", requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y, _ = Fn.gated_scan(z, lengths=torch.tensor([20, 3], dtype=torch.int32, device="cuda"))
+        with pytest.raises(RuntimeError, match=message):
+            torch.autograd.grad(y.sum(), z)
