@@ -95,7 +95,8 @@ std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& z, const Tensor& h
     const c10::DeviceGuard guard(z.device());
     const ScanShape s = scan_shape(z, gated);
     Tensor y;
-    if (s.B > 1 && s.T > 1 && z.stride(0) < z.stride(1)) y = at::empty({s.T, s.B, s.D}, z.options()).transpose(0, 1);
+    // in z's order, and no view: the results of an autograd node may then be modified in place
+    if (s.B > 1 && s.T > 1 && z.stride(0) < z.stride(1)) y = at::empty_strided({s.B, s.T, s.D}, {s.D, s.B * s.D, 1}, z.options());
     else y = at::empty({s.B, s.T, s.D}, z.options());
     Tensor h_last = at::empty({s.B, s.D}, z.options().dtype(at::kFloat)), kept;
     if (track) kept = bytes(s.kept + (int8 ? s.codes : 0), z);

@@ -79,3 +79,31 @@ def test_saved_tensors_that_come_back_as_others_are_refused(unpack, message):
         y, _ = Fn.gated_scan(z, lengths=torch.tensor([20, 3], dtype=torch.int32, device="cuda"))
         with pytest.raises(RuntimeError, match=message):
             torch.autograd.grad(y.sum(), z)
+
+
+@pytest.mark.parametrize("save", ["input", "int8"])
+@pytest.mark.parametrize("layout", ["batch", "time"])
+def test_scan_results_are_modified_in_place(layout, save):
+    """A layer that goes on in place (dropout mask, residual) gives the gradients of the one that does not."""
+    torch, Fn = _t()
+    torch.manual_seed(5)
+    B, T, D = 4, 21, 24
+    z = torch.randn(B, T, 3 * D, device="cuda")
+    if layout == "time":
+        z = z.transpose(0, 1).contiguous().transpose(0, 1)
+    z.requires_grad_(True)
+    res = torch.randn(B, T, D, device="cuda", requires_grad=True)
+    keep = (torch.rand(B, T, D, device="cuda") > 0.3).float()
+    grads = []
+    for inplace in (True, False):
+        y, last = Fn.gated_scan(z, save=save)
+        if inplace:
+            y.mul_(keep)
+            y += res
+            last.mul_(2.0)
+        else:
+            y, last = y * keep + res, last * 2.0
+        grads.append((y.detach(),) + torch.autograd.grad(y.square().sum() + last.square().sum(), [z, res]))
+        assert (y.stride(0) < y.stride(1)) == (layout == "time")
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
