@@ -282,12 +282,19 @@ Tensor linear_rows(const Tensor& x, const Tensor& w, const OptTensor& b) {
     return swap ? y.view(lead).transpose(0, 1) : y.view(lead);
 }
 
+// The same where no derivative is taken through it: its result is no view for autograd, so that it may be modified in place
+// (views made inside an autograd node or under no_grad may not).
+Tensor linear_rows_fresh(const Tensor& x, const Tensor& w, const OptTensor& b) {
+    const at::AutoDispatchBelowADInplaceOrView guard;
+    return linear_rows(x, w, b);
+}
+
 struct Linear8 : torch::autograd::Function<Linear8> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias) {
         const Tensor w = weight.to(x.scalar_type());
         OptTensor b;
         if (bias.has_value()) b = bias->to(x.scalar_type());
-        Tensor y = linear_rows(x, w, b), saved;
+        Tensor y = linear_rows_fresh(x, w, b), saved;
         const bool keep = weight.requires_grad() || (bias.has_value() && bias->requires_grad());
         if (keep) saved = checkpoint8(x);
         ctx->save_for_backward({x.requires_grad() ? w : Tensor(), saved});
@@ -318,7 +325,10 @@ Tensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
         return Linear8::apply(x, weight, bias);
     OptTensor b;
     if (bias.has_value()) b = bias->to(x.scalar_type());
-    return linear_rows(x, weight.to(x.scalar_type()), b);
+    const Tensor w = weight.to(x.scalar_type());
+    const auto dual = [](const Tensor& t) { return t._fw_grad(0).defined(); };
+    if (dual(x) || dual(w) || (b.has_value() && dual(*b))) return linear_rows(x, w, b);      // forward-mode derivative
+    return linear_rows_fresh(x, w, b);
 }
 
 }  // namespace

@@ -107,3 +107,46 @@ def test_scan_results_are_modified_in_place(layout, save):
         assert (y.stride(0) < y.stride(1)) == (layout == "time")
     for a, b in zip(*grads):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("layout,shape", [("batch", (6, 20)), ("batch", (20,)), ("batch", (4, 6, 20)), ("time", (4, 6, 20)),
+                                          ("batch", (2, 3, 5, 20))], ids=str)
+def test_linear8_result_is_modified_in_place(layout, shape):
+    torch, Fn = _t()
+    torch.manual_seed(6)
+    x = torch.randn(shape, device="cuda")
+    if layout == "time":
+        x = x.transpose(0, 1).contiguous().transpose(0, 1)
+    x.requires_grad_(True)
+    w, b = torch.randn(7, 20, device="cuda", requires_grad=True), torch.randn(7, device="cuda", requires_grad=True)
+    res = torch.randn(shape[:-1] + (7,), device="cuda", requires_grad=True)
+    grads = []
+    for inplace in (True, False):
+        y = Fn.linear8(x, w, b)
+        if inplace:
+            y.mul_(2.0)
+            y += res
+        else:
+            y = y * 2.0 + res
+        grads.append((y.detach(),) + torch.autograd.grad(y.square().sum(), [x, w, b, res]))
+    for a, c in zip(*grads):
+        assert torch.equal(a, c)
+    with torch.no_grad():
+        y = Fn.linear8(x, w, b)
+    y += res                                            # made without a graph, modified with one
+    assert torch.equal(torch.autograd.grad(y.sum(), res)[0], torch.ones_like(res))
+
+
+@pytest.mark.parametrize("layout", ["batch", "time"])
+def test_linear8_forward_derivative_without_a_graph(layout):
+    """A dual tensor that needs no gradient: y is linear in it, and keeps its tangent."""
+    torch, Fn = _t()
+    import torch.autograd.forward_ad as fa
+    g = torch.Generator().manual_seed(8)
+    x, t = (torch.randint(-3, 4, (4, 6, 20), generator=g).float().cuda() for _ in range(2))      # exact in any order
+    w = torch.randint(-3, 4, (7, 20), generator=g).float().cuda()
+    if layout == "time":
+        x, t = (v.transpose(0, 1).contiguous().transpose(0, 1) for v in (x, t))
+    with fa.dual_level():
+        y = fa.unpack_dual(Fn.linear8(fa.make_dual(x, t), w))
+        assert torch.equal(y.primal, x @ w.t()) and torch.equal(y.tangent, t @ w.t())
