@@ -277,7 +277,8 @@ Tensor linear_rows(const Tensor& x, const Tensor& w, const OptTensor& b) {
     const bool swap = x.dim() == 3 && !x.is_contiguous() && x.transpose(0, 1).is_contiguous();
     const Tensor xt = swap ? x.transpose(0, 1) : x;
     auto lead = xt.sizes().vec();
-    const Tensor y = at::linear(xt.reshape({-1, x.size(-1)}), w, b);
+    const int64_t rows = c10::multiply_integers(lead.begin(), lead.end() - 1);      // x may have no channels
+    const Tensor y = at::linear(xt.reshape({rows, x.size(-1)}), w, b);
     lead.back() = w.size(0);
     return swap ? y.view(lead).transpose(0, 1) : y.view(lead);
 }

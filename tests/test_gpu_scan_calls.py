@@ -150,3 +150,17 @@ def test_linear8_forward_derivative_without_a_graph(layout):
     with fa.dual_level():
         y = fa.unpack_dual(Fn.linear8(fa.make_dual(x, t), w))
         assert torch.equal(y.primal, x @ w.t()) and torch.equal(y.tangent, t @ w.t())
+
+
+@pytest.mark.parametrize("rows,K,N", [((2, 3), 0, 5), ((2, 3), 4, 0), ((), 0, 5), ((2, 0), 4, 5), ((0,), 0, 0)], ids=str)
+def test_linear8_with_an_empty_axis(rows, K, N):
+    """As the linear layer: no input channel gives the bias, no output channel and no row give empty results."""
+    torch, Fn = _t()
+    x, w = torch.ones(rows + (K,), device="cuda", requires_grad=True), torch.ones(N, K, device="cuda", requires_grad=True)
+    b = torch.arange(N, dtype=torch.float32, device="cuda").requires_grad_(True)
+    out = []
+    for f in (Fn.linear8, torch.nn.functional.linear):
+        y = f(x, w, b)
+        out.append((y,) + torch.autograd.grad(y.sum(), [x, w, b]))
+    for a, c in zip(*out):
+        assert a.shape == c.shape and torch.equal(a, c)
