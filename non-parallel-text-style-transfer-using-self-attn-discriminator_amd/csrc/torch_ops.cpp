@@ -69,6 +69,12 @@ variable_list once(variable_list grads, const char* name) {
     return (*fn)(std::move(grads));
 }
 
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+// the kernels write no tangents: a dual tensor's derivative would count as zero
+void no_tangent(const char* name, const Tensor& a, const Tensor& b, const Tensor& c = Tensor()) {
+    TORCH_CHECK(!dual(a) && !dual(b) && !dual(c), name, " has no forward-mode derivative");
+}
+
 // sizes go into 32-bit fields
 int dim32(int64_t n) {
     TORCH_CHECK(n <= INT32_MAX, "a size of ", n, " is beyond the supported maximum");
@@ -179,6 +185,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 };
 
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& z, const OptTensor& h0, const OptTensor& lengths, bool reverse, bool gated, bool int8) {
+    no_tangent("gated_scan", z, h0.value_or(Tensor()));
     if (at::GradMode::is_enabled() && (z.requires_grad() || (h0.has_value() && h0->requires_grad()))) {
         auto r = GatedScan::apply(z, h0, lengths, reverse, gated, int8);
         return {r[0], r[1]};
@@ -189,6 +196,7 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& z, const OptTensor& h0, cons
 
 // y; the new states go to h_out (h itself updates in place)
 Tensor gated_scan_step(const Tensor& z, const Tensor& h, const OptTensor& alive, bool gated, const Tensor& h_out) {
+    no_tangent("gated_scan_step", z, h, h_out);
     const c10::DeviceGuard guard(z.device());
     Tensor y = at::empty({h.size(0), h.size(1)}, z.options());
     if (h.size(0) == 0) return y;
@@ -327,8 +335,7 @@ Tensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
     OptTensor b;
     if (bias.has_value()) b = bias->to(x.scalar_type());
     const Tensor w = weight.to(x.scalar_type());
-    const auto dual = [](const Tensor& t) { return t._fw_grad(0).defined(); };
-    if (dual(x) || dual(w) || (b.has_value() && dual(*b))) return linear_rows(x, w, b);      // forward-mode derivative
+    if (dual(x) || dual(w) || dual(b.value_or(Tensor()))) return linear_rows(x, w, b);      // forward-mode derivative
     return linear_rows_fresh(x, w, b);
 }
 

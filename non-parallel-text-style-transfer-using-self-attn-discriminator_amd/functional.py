@@ -729,7 +729,7 @@ def gated_scan(z, h0=None, lengths=None, reverse=False, gated_output=True, save=
     long text can be read in pieces.  ``lengths`` [B] (host or device, 0..T, any order): y is 0 at t >= length, the state
     stays, and such rows of z may hold anything.  ``reverse`` runs from the last token to the first.
 
-    Differentiable in z and h0.  ``save="input"`` keeps z for the backward pass; ``save="int8"`` keeps its 8-bit codes
+    Differentiable in z and h0, once and in reverse mode (dual tensors are refused).  ``save="input"`` keeps z for the backward pass; ``save="int8"`` keeps its 8-bit codes
     instead (``checkpoint8``'s format, x, f and o separately) and gives the gradient at the restored values; both keep the
     state entering every 16 tokens in float32, and a step between them is recomputed from there."""
     _kind(z, "z")
@@ -773,7 +773,7 @@ def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
 
     ``z`` [B,3D] / [B,2D] are the token's pre-activations, ``h`` [B,D] float32 the states.  The new states go to ``h_out``
     (a new tensor if None; ``h`` itself updates in place).  ``alive`` [B] bool: a sentence that has ended keeps its state
-    and gives y = 0.  No gradient (train with ``gated_scan``)."""
+    and gives y = 0.  No gradient, and dual tensors are refused (train with ``gated_scan``)."""
     _kind(z, "z")
     if z.dim() != 2:
         raise RuntimeError("z must be [B,3D] or [B,2D], got %s" % (tuple(z.shape),))
@@ -818,7 +818,7 @@ def checkpoint8(x):
     """Keep ``x`` [..., C] (float32 / bfloat16 / float16) in 8 bits: int8 codes with one power-of-two step per row and 32
     channels, the smallest whose 127 steps reach the largest finite entry.  An entry comes back within half a step (at most
     1/127 of that largest entry; 1/63 where the type's own largest values leave no room above); infinities and NaN come
-    back as NaN and leave their neighbours alone.  Returns a ``Checkpoint8``; no gradient flows through it."""
+    back as NaN and leave their neighbours alone.  Returns a ``Checkpoint8``; no derivative of either mode flows through it."""
     _kind(x, "x")
     if x.dim() == 0:
         raise RuntimeError("x must have a channel axis")
@@ -829,7 +829,7 @@ def checkpoint8(x):
 def weight_grad8(dy, ckpt, bias=False):
     """Weight gradient ``dW [N,K] = dy^T x^`` (float32) of a linear layer from the checkpoint of its input ``x`` [..., K];
     ``dy`` [..., N] has x's leading shape and type.  ``bias=True`` adds ``db [N] = sum dy``: ``(dW, db)``.  Sums are
-    float32 in a fixed order: the same call gives the same bits."""
+    float32 in a fixed order: the same call gives the same bits.  dy counts as a constant: no derivative flows through it."""
     _kind(dy, "dy")
     if dy.dtype != ckpt.dtype or dy.dim() != len(ckpt.shape) or dy.shape[:-1] != ckpt.shape[:-1]:
         raise RuntimeError("dy %s %s does not belong to a checkpoint of %s %s"

@@ -164,3 +164,19 @@ def test_linear8_with_an_empty_axis(rows, K, N):
         out.append((y,) + torch.autograd.grad(y.sum(), [x, w, b]))
     for a, c in zip(*out):
         assert a.shape == c.shape and torch.equal(a, c)
+
+
+def test_dual_tensors_are_refused_where_a_tangent_would_be_lost():
+    torch, Fn = _t()
+    import torch.autograd.forward_ad as fa
+    with fa.dual_level():
+        z = fa.make_dual(torch.zeros(2, 3, 12, device="cuda"), torch.ones(2, 3, 12, device="cuda"))
+        h = torch.zeros(2, 4, device="cuda")
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            Fn.gated_scan(z)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            Fn.gated_scan(z, save="int8")
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            Fn.gated_scan_step(z[:, 0], h)
+        assert not h.any()
+        assert not Fn.gated_scan(fa.unpack_dual(z).primal)[0].any()

@@ -39,3 +39,24 @@ def test_weight_gradient_takes_whole_checkpoints_on_the_device_only(saved, messa
         lib.load_ops().weight_grad8(torch.zeros(4, 5), saved, 6, True)
     with pytest.raises(RuntimeError):
         Fn.weight_grad8(torch.zeros(4, 5), Fn.Checkpoint8(saved, (4, 6), F32), bias=True)
+
+
+@pytest.mark.parametrize("which", ["z", "h0"])
+def test_scan_refuses_dual_tensors(which):
+    import torch.autograd.forward_ad as fa
+    ops, args = lib.load_ops(), dict(z=torch.zeros(2, 3, 12), h0=torch.zeros(2, 4))
+    with fa.dual_level():
+        args[which] = fa.make_dual(args[which], torch.ones_like(args[which]))
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="gated_scan has no forward-mode derivative"):
+                ops.gated_scan(args["z"], args["h0"], None, False, True, False)
+
+
+@pytest.mark.parametrize("which", ["z", "h", "h_out"])
+def test_step_refuses_dual_tensors(which):
+    import torch.autograd.forward_ad as fa
+    args = dict(z=torch.zeros(2, 12), h=torch.zeros(2, 4), h_out=torch.zeros(2, 4))
+    with fa.dual_level(), torch.no_grad():
+        args[which] = fa.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(RuntimeError, match="gated_scan_step has no forward-mode derivative"):
+            lib.load_ops().gated_scan_step(args["z"], args["h"], None, True, args["h_out"])
