@@ -779,7 +779,7 @@ def gated_scan_step(z, h, alive=None, gated_output=True, h_out=None):
         raise RuntimeError("z must be [B,3D] or [B,2D], got %s" % (tuple(z.shape),))
     D = _scan_parts(z.shape[1], gated_output)
     B, dev = z.shape[0], z.device
-    if torch.is_grad_enabled() and (z.requires_grad or h.requires_grad):
+    if torch.is_grad_enabled() and (z.requires_grad or h.requires_grad or (h_out is not None and h_out.requires_grad)):
         raise RuntimeError("gated_scan_step has no gradient: call it under torch.no_grad(), or train with gated_scan")
     _need_state(h, "h", B, D, dev)
     if alive is not None and (alive.dtype not in (torch.bool, torch.uint8) or tuple(alive.shape) != (B,) or alive.device != dev):

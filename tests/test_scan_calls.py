@@ -60,3 +60,11 @@ def test_step_refuses_dual_tensors(which):
         args[which] = fa.make_dual(args[which], torch.ones_like(args[which]))
         with pytest.raises(RuntimeError, match="gated_scan_step has no forward-mode derivative"):
             lib.load_ops().gated_scan_step(args["z"], args["h"], None, True, args["h_out"])
+
+
+def test_step_refuses_to_write_into_a_tensor_that_needs_a_gradient():
+    h_out = torch.zeros(2, 4, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        Fn.gated_scan_step(torch.zeros(2, 12), torch.zeros(2, 4), h_out=h_out)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):      # past that check
+        Fn.gated_scan_step(torch.zeros(2, 12), torch.zeros(2, 4), h_out=h_out)
