@@ -146,6 +146,15 @@ def pack_weights(params, V=None, E=None, H=None, L=None, cell=_lib.CELL_LSTM, up
     return pw
 
 
+def _own_int32(host):
+    """An int32 copy of a host tensor: from pinned memory the transfer to the device runs after the call has returned, when the
+    caller may have filled the buffer with the next batch's values.  The copy is pinned where the source is (torch's host
+    allocator keeps it until the transfer is done), so that the call waits for the stream no more than before."""
+    if not host.is_pinned():
+        return host.detach().to(torch.int32, copy=True)
+    return torch.empty(host.shape, dtype=torch.int32, pin_memory=True).copy_(host.detach())
+
+
 def _lengths_to_device(src_len, B, device):
     """Reference callers pass CPU int16/int32/int64 lengths (transfer/models.py:1172, utils/data.py:84);
     sortedness is what ``pack_padded_sequence(enforce_sorted=True)`` enforces (transfer/models.py:904)."""
@@ -710,6 +719,7 @@ def _scan_lengths(lengths, B, T, dev):
         ln = lengths.detach().numpy()
         if B > 0 and (int(ln.min()) < 0 or int(ln.max()) > T):
             raise RuntimeError("lengths must lie in 0..%d, got %d..%d" % (T, int(ln.min()), int(ln.max())))
+        lengths = _own_int32(lengths)
     elif lengths.device != dev:
         raise RuntimeError("lengths are on %s, z is on %s" % (lengths.device, dev))
     elif lengths.dtype == torch.int64:

@@ -180,3 +180,20 @@ def test_dual_tensors_are_refused_where_a_tangent_would_be_lost():
             Fn.gated_scan_step(z[:, 0], h)
         assert not h.any()
         assert not Fn.gated_scan(fa.unpack_dual(z).primal)[0].any()
+
+
+def test_pinned_lengths_may_be_refilled_after_the_call():
+    """The copy to the device waits behind earlier work on the stream; the caller's buffer is free as soon as the call is back."""
+    torch, Fn = _t()
+    torch.manual_seed(7)
+    z = torch.randn(3, 40, 3 * 16, device="cuda")
+    lengths = torch.tensor([40, 7, 0], dtype=torch.int32).pin_memory()
+    want = Fn.gated_scan(z, lengths=[40, 7, 0])
+    a = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(40):
+        a = (a @ a) * 1e-3                       # some milliseconds of work in front
+    got = Fn.gated_scan(z, lengths=lengths)
+    lengths.fill_(1)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

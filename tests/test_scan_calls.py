@@ -68,3 +68,12 @@ def test_step_refuses_to_write_into_a_tensor_that_needs_a_gradient():
         Fn.gated_scan_step(torch.zeros(2, 12), torch.zeros(2, 4), h_out=h_out)
     with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):      # past that check
         Fn.gated_scan_step(torch.zeros(2, 12), torch.zeros(2, 4), h_out=h_out)
+
+
+@pytest.mark.parametrize("dtype", [torch.int16, torch.int32, torch.int64])
+def test_host_lengths_are_copied_before_the_call_returns(dtype):
+    """What goes to the device is no alias of the caller's buffer (with the host in the device's place it would show)."""
+    buf = torch.tensor([3, 0, 2], dtype=dtype)
+    sent = Fn._scan_lengths(buf, 3, 3, torch.device("cpu"))
+    buf.zero_()
+    assert sent.tolist() == [3, 0, 2] and sent.dtype == torch.int32
