@@ -715,7 +715,7 @@ def _scan_lengths(lengths, B, T, dev):
         lengths = torch.as_tensor(lengths)
     if lengths.dtype == torch.int32 and lengths.is_cuda and lengths.shape == (B,) and lengths.device == dev:
         return lengths.contiguous()
-    if lengths.dim() != 1 or lengths.numel() != B or lengths.dtype.is_floating_point or lengths.dtype in (torch.bool, torch.complex64):
+    if lengths.dim() != 1 or lengths.numel() != B or lengths.dtype.is_floating_point or lengths.dtype.is_complex or lengths.dtype == torch.bool:
         raise RuntimeError("lengths must be %d integers, got %s of shape %s" % (B, lengths.dtype, tuple(lengths.shape)))
     if not lengths.is_cuda:
         ln = lengths.detach().numpy()
@@ -724,8 +724,8 @@ def _scan_lengths(lengths, B, T, dev):
         lengths = _own_int32(lengths)
     elif lengths.device != dev:
         raise RuntimeError("lengths are on %s, z is on %s" % (lengths.device, dev))
-    elif lengths.dtype == torch.int64:
-        lengths = lengths.clamp(0, T)               # before it is narrowed
+    elif lengths.dtype.itemsize > 4 or lengths.dtype == torch.uint32:
+        lengths = lengths.to(torch.int64).clamp(0, T)               # before it is narrowed
     return lengths.to(device=dev, dtype=torch.int32, non_blocking=True).contiguous()
 
 

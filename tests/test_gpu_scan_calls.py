@@ -197,3 +197,14 @@ def test_pinned_lengths_may_be_refilled_after_the_call():
     lengths.fill_(1)
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", ["uint8", "int16", "uint32", "int64"])
+def test_device_lengths_of_any_integer_type_are_clamped(dtype):
+    torch, Fn = _t()
+    torch.manual_seed(2)
+    z = torch.randn(3, 20, 3 * 8, device="cuda")
+    top = {"uint8": 255, "int16": 2 ** 15 - 1, "uint32": 2 ** 32 - 1, "int64": 2 ** 40 + 1}[dtype]
+    lengths = torch.tensor([top, 7, 0], dtype=torch.int64).to(getattr(torch, dtype)).cuda()
+    for a, b in zip(Fn.gated_scan(z, lengths=lengths), Fn.gated_scan(z, lengths=[20, 7, 0])):
+        assert torch.equal(a, b)

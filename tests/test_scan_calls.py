@@ -77,3 +77,9 @@ def test_host_lengths_are_copied_before_the_call_returns(dtype):
     sent = Fn._scan_lengths(buf, 3, 3, torch.device("cpu"))
     buf.zero_()
     assert sent.tolist() == [3, 0, 2] and sent.dtype == torch.int32
+
+
+@pytest.mark.parametrize("dtype", [torch.complex32, torch.complex64, torch.complex128, torch.float64, torch.bool])
+def test_lengths_are_integers(dtype):
+    with pytest.raises(RuntimeError, match="must be 2 integers"):
+        Fn.gated_scan(torch.zeros(2, 3, 12), lengths=torch.ones(2).to(dtype))
