@@ -69,6 +69,30 @@ variable_list once(variable_list grads, const char* name) {
     return (*fn)(std::move(grads));
 }
 
+// The kernels follow data pointers: every tensor has to have memory on the device.  Fake and meta tensors (tracing) and the
+// wrappers of function transforms have none.
+void need_memory(const Tensor& t, const char* name, const char* what) {
+    TORCH_CHECK(t.has_storage() && t.storage().device_type() != at::kMeta, name, ": ", what,
+                " has no memory (a meta or fake tensor, or the wrapper of a function transform); the operator cannot be traced");
+    TORCH_CHECK(t.is_cuda(), name, ": ", what, " must be on the HIP device, got ", t.device(), "; there is no CPU path");
+}
+void need_matrix(const Tensor& t, const char* name, const char* what, at::ScalarType type, int64_t rows, int64_t cols, at::Device device) {
+    need_memory(t, name, what);
+    TORCH_CHECK(t.scalar_type() == type && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1 && t.device() == device,
+                name, ": ", what, " must be ", type, " [", rows, ",", cols, "] with unit channel stride on ", device);
+}
+void need_vector(const Tensor& t, const char* name, const char* what, int64_t n, at::Device device) {
+    need_memory(t, name, what);
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == n && t.device() == device, name, ": ", what, " must hold ", n, " entries on ", device);
+}
+int64_t channels_of(const Tensor& z, const char* name, int64_t dim, bool gated) {
+    need_memory(z, name, "z");
+    const int64_t parts = gated ? 3 : 2;
+    TORCH_CHECK(z.dim() == dim && z.size(-1) % parts == 0 && z.size(-1) >= 2 * parts, name, ": z must hold ", parts, " parts of two channels or more, got ",
+                z.sizes());
+    return z.size(-1) / parts;
+}
+
 bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 // the kernels write no tangents: a dual tensor's derivative would count as zero
 void no_tangent(const char* name, const Tensor& a, const Tensor& b, const Tensor& c = Tensor()) {
@@ -186,6 +210,16 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& z, const OptTensor& h0, const OptTensor& lengths, bool reverse, bool gated, bool int8) {
     no_tangent("gated_scan", z, h0.value_or(Tensor()));
+    const int64_t D = channels_of(z, "gated_scan", 3, gated);
+    TORCH_CHECK(z.stride(2) == 1, "gated_scan: z must have unit channel stride");
+    if (h0.has_value()) {
+        need_matrix(*h0, "gated_scan", "h0", at::kFloat, z.size(0), D, z.device());
+        TORCH_CHECK(h0->is_contiguous(), "gated_scan: h0 must be contiguous");
+    }
+    if (lengths.has_value()) {
+        need_vector(*lengths, "gated_scan", "lengths", z.size(0), z.device());
+        TORCH_CHECK(lengths->scalar_type() == at::kInt && lengths->is_contiguous(), "gated_scan: lengths must be contiguous int32");
+    }
     if (at::GradMode::is_enabled() && (z.requires_grad() || (h0.has_value() && h0->requires_grad()))) {
         auto r = GatedScan::apply(z, h0, lengths, reverse, gated, int8);
         return {r[0], r[1]};
@@ -197,6 +231,13 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& z, const OptTensor& h0, cons
 // y; the new states go to h_out (h itself updates in place)
 Tensor gated_scan_step(const Tensor& z, const Tensor& h, const OptTensor& alive, bool gated, const Tensor& h_out) {
     no_tangent("gated_scan_step", z, h, h_out);
+    const int64_t D = channels_of(z, "gated_scan_step", 2, gated);
+    need_matrix(h, "gated_scan_step", "h", at::kFloat, z.size(0), D, z.device());
+    need_matrix(h_out, "gated_scan_step", "h_out", at::kFloat, z.size(0), D, z.device());
+    if (alive.has_value()) {
+        need_vector(*alive, "gated_scan_step", "alive", z.size(0), z.device());
+        TORCH_CHECK(alive->scalar_type() == at::kBool || alive->scalar_type() == at::kByte, "gated_scan_step: alive must be bool");
+    }
     const c10::DeviceGuard guard(z.device());
     Tensor y = at::empty({h.size(0), h.size(1)}, z.options());
     if (h.size(0) == 0) return y;
@@ -224,6 +265,8 @@ Rows rows_of(Tensor t) {
 
 // 8-bit checkpoint of x [..., C]
 Tensor checkpoint8(const Tensor& x) {
+    TORCH_CHECK(x.dim() > 0, "checkpoint8: x must have a channel axis");
+    need_memory(x, "checkpoint8", "x");
     const c10::DeviceGuard guard(x.device());
     if (x.numel() == 0) return bytes(0, x);
     const Rows r = rows_of(x.detach());
@@ -239,7 +282,7 @@ void need_saved(const Tensor& saved, int64_t rows, int64_t C) {
                 saved.is_contiguous() ? "" : " (not contiguous)");
     const size_t n = rows > 0 && C > 0 ? size_of(api.ckpt_bytes(rows, C), "sad_checkpoint8_bytes") : 0;
     TORCH_CHECK((size_t)saved.numel() == n, "a checkpoint of ", rows, " x ", C, " entries holds ", n, " bytes, got ", saved.numel());
-    TORCH_CHECK(saved.is_cuda(), "a checkpoint's codes must be on the HIP device, got ", saved.device(), "; there is no CPU path");
+    need_memory(saved, "a checkpoint", "saved");
 }
 
 // the values a checkpoint stands for, contiguous
@@ -260,6 +303,7 @@ std::tuple<Tensor, Tensor> weight_grad8(const Tensor& dy, const Tensor& saved, i
     TORCH_CHECK(dy.dim() > 0, "dy must have a channel axis");
     const int64_t rows = c10::multiply_integers(dy.sizes().slice(0, dy.dim() - 1));
     need_saved(saved, rows, K);
+    need_memory(dy, "weight_grad8", "dy");
     TORCH_CHECK(saved.device() == dy.device(), "dy is on ", dy.device(), ", the checkpoint on ", saved.device());
     const c10::DeviceGuard guard(dy.device());
     if (dy.numel() == 0 || K == 0) {
@@ -330,6 +374,11 @@ struct Linear8 : torch::autograd::Function<Linear8> {
 };
 
 Tensor linear8(const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+    need_memory(x, "linear8", "x");
+    need_memory(weight, "linear8", "weight");
+    TORCH_CHECK(x.dim() > 0 && weight.dim() == 2 && x.size(-1) == weight.size(1) && weight.device() == x.device(), "linear8: x ", x.sizes(),
+                " and weight ", weight.sizes(), " do not fit");
+    if (bias.has_value()) need_vector(*bias, "linear8", "bias", weight.size(0), x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias.has_value() && bias->requires_grad())))
         return Linear8::apply(x, weight, bias);
     OptTensor b;

@@ -208,3 +208,29 @@ def test_device_lengths_of_any_integer_type_are_clamped(dtype):
     lengths = torch.tensor([top, 7, 0], dtype=torch.int64).to(getattr(torch, dtype)).cuda()
     for a, b in zip(Fn.gated_scan(z, lengths=lengths), Fn.gated_scan(z, lengths=[20, 7, 0])):
         assert torch.equal(a, b)
+
+
+def test_operators_check_their_own_arguments():
+    """torch.ops.sad_amd is public: what the kernels assume is checked there too."""
+    torch, Fn = _t()
+    from sad_amd import lib
+    ops = lib.load_ops()
+    f = lambda *shape, dtype=torch.float32: torch.zeros(shape, dtype=dtype, device="cuda")
+    scan = lambda z=f(2, 3, 12), h0=None, lengths=None: ops.gated_scan(z, h0, lengths, False, True, False)
+    step = lambda z=f(2, 12), h=f(2, 4), alive=None, h_out=f(2, 4): ops.gated_scan_step(z, h, alive, True, h_out)
+    scan(), step()
+    for call, message in (
+        (lambda: scan(f(2, 3, 13)), "parts of two channels"), (lambda: scan(f(2, 12)), "parts of two channels"),
+        (lambda: scan(f(2, 12, 3).transpose(1, 2)), "unit channel stride"), (lambda: scan(f(2, 3, 12, dtype=torch.float64)), "expected float32"),
+        (lambda: scan(h0=f(1, 4)), "h0 must be"), (lambda: scan(h0=f(2, 4, dtype=torch.float16)), "h0 must be"),
+        (lambda: scan(h0=f(2, 8)[:, :4]), "h0 must be contiguous"), (lambda: scan(h0=torch.zeros(2, 4)), "HIP device"),
+        (lambda: scan(lengths=f(3, dtype=torch.int32)), "lengths must hold 2"), (lambda: scan(lengths=f(2, dtype=torch.int64)), "int32"),
+        (lambda: scan(lengths=torch.zeros(2, dtype=torch.int32)), "HIP device"),
+        (lambda: step(h=f(2, 3)), "h must be"), (lambda: step(h_out=f(4, 2).t()), "h_out must be"), (lambda: step(h=torch.zeros(2, 4)), "HIP device"),
+        (lambda: step(alive=f(2)), "alive must be"), (lambda: step(alive=f(1, dtype=torch.bool)), "alive must hold"),
+        (lambda: ops.linear8(f(3, 5), f(2, 4), None), "do not fit"), (lambda: ops.linear8(f(3, 5), f(2, 5), f(3)), "bias must hold"),
+        (lambda: ops.linear8(f(3, 5), torch.zeros(2, 5), None), "HIP device"),
+        (lambda: ops.checkpoint8(f(2, 3, dtype=torch.int32)), "expected float32"),
+    ):
+        with pytest.raises(RuntimeError, match=message):
+            call()

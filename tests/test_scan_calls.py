@@ -83,3 +83,48 @@ def test_host_lengths_are_copied_before_the_call_returns(dtype):
 def test_lengths_are_integers(dtype):
     with pytest.raises(RuntimeError, match="must be 2 integers"):
         Fn.gated_scan(torch.zeros(2, 3, 12), lengths=torch.ones(2).to(dtype))
+
+
+def _direct(device="cpu"):
+    """Calls of the operators themselves, past functional's checks."""
+    ops = lib.load_ops()
+    f = lambda *shape, dtype=F32: torch.zeros(shape, dtype=dtype, device=device)
+    return {
+        "gated_scan": lambda: ops.gated_scan(f(2, 3, 12), f(2, 4), f(2, dtype=torch.int32), False, True, False),
+        "gated_scan int8": lambda: ops.gated_scan(f(2, 3, 12).requires_grad_(True), None, None, False, True, True),
+        "gated_scan_step": lambda: ops.gated_scan_step(f(2, 12), f(2, 4), None, True, f(2, 4)),
+        "checkpoint8": lambda: ops.checkpoint8(f(3, 5)),
+        "restore8": lambda: ops.restore8(f(3 * 34, dtype=torch.uint8), [3, 5], F32),
+        "weight_grad8": lambda: ops.weight_grad8(f(3, 2), f(3 * 34, dtype=torch.uint8), 5, True),
+        "linear8": lambda: ops.linear8(f(3, 5), f(2, 5), f(2)),
+        "linear8 grad": lambda: ops.linear8(f(3, 5).requires_grad_(True), f(2, 5), f(2)),
+    }
+
+
+@pytest.mark.parametrize("name", sorted(_direct()))
+def test_operators_refuse_host_tensors(name):
+    with pytest.raises(RuntimeError, match="must be on the HIP device"):
+        _direct()[name]()
+
+
+@pytest.mark.parametrize("device", ["cuda", "cpu"])
+@pytest.mark.parametrize("name", sorted(_direct()))
+def test_operators_refuse_fake_tensors(name, device):
+    """A tracer's tensors have no memory: nothing may follow their pointers or trace a call without its work."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(), pytest.raises(RuntimeError, match="cannot be traced"):
+        _direct(device=device)[name]()
+
+
+@pytest.mark.parametrize("name", sorted(_direct()))
+def test_operators_refuse_meta_tensors(name):
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        _direct(device="meta")[name]()
+
+
+def test_operators_refuse_the_wrappers_of_function_transforms():
+    ops = lib.load_ops()
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.func.grad(lambda x: ops.linear8(x, torch.zeros(2, 5), None).sum())(torch.zeros(3, 5))
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.func.grad(lambda z: ops.gated_scan(z, None, None, False, True, False)[0].sum())(torch.zeros(2, 3, 12))
