@@ -14,6 +14,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <cstring>
+#include <dlfcn.h>
+
 #include "../../include/sad.h"
 
 namespace {
@@ -38,13 +41,34 @@ struct Api {
     decltype(&sad_weight_grad8) wgrad = nullptr;
 } api;
 
-// addresses in the order of Api's members
+// Addresses in the order of Api's members.  The operator is public and its arguments are numbers: each has to be where a
+// loaded library exports the function of that name.
 void bind(at::IntArrayRef a) {
     TORCH_CHECK(a.size() == 12, "expected 12 addresses");
+    auto look = [&](int i, const char* name) {
+        Dl_info info{};
+        void* p = reinterpret_cast<void*>(a[i]);
+        TORCH_CHECK(dladdr(p, &info) != 0 && info.dli_saddr == p && info.dli_sname != nullptr && std::strcmp(info.dli_sname, name) == 0,
+                    "address ", i, " is not ", name);
+        return p;
+    };
+    Api next;
     int i = 0;
-    auto take = [&](auto& f) { f = reinterpret_cast<std::decay_t<decltype(f)>>(a[i++]); };
-    take(api.last_error); take(api.scan_ws); take(api.scan_kept); take(api.scan_codes); take(api.scan_fwd); take(api.scan_bwd);
-    take(api.scan_step); take(api.ckpt_bytes); take(api.ckpt_save); take(api.ckpt_restore); take(api.wgrad_ws); take(api.wgrad);
+#define SAD_TAKE(member, name) next.member = reinterpret_cast<decltype(next.member)>(look(i++, #name))
+    SAD_TAKE(last_error, sad_last_error);
+    SAD_TAKE(scan_ws, sad_gated_scan_workspace_bytes);
+    SAD_TAKE(scan_kept, sad_gated_scan_kept_bytes);
+    SAD_TAKE(scan_codes, sad_gated_scan_codes_bytes);
+    SAD_TAKE(scan_fwd, sad_gated_scan_fwd);
+    SAD_TAKE(scan_bwd, sad_gated_scan_bwd);
+    SAD_TAKE(scan_step, sad_gated_scan_step);
+    SAD_TAKE(ckpt_bytes, sad_checkpoint8_bytes);
+    SAD_TAKE(ckpt_save, sad_checkpoint8_save);
+    SAD_TAKE(ckpt_restore, sad_checkpoint8_restore);
+    SAD_TAKE(wgrad_ws, sad_weight_grad8_workspace_bytes);
+    SAD_TAKE(wgrad, sad_weight_grad8);
+#undef SAD_TAKE
+    api = next;
 }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, "libsad ", what, " failed (", rc, "): ", api.last_error()); }

@@ -128,3 +128,20 @@ def test_operators_refuse_the_wrappers_of_function_transforms():
         torch.func.grad(lambda x: ops.linear8(x, torch.zeros(2, 5), None).sum())(torch.zeros(3, 5))
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.func.grad(lambda z: ops.gated_scan(z, None, None, False, True, False)[0].sum())(torch.zeros(2, 3, 12))
+
+
+def test_bind_takes_the_library_s_own_functions_only():
+    import ctypes
+    ops, l = lib.load_ops(), lib.load()
+    names = ("sad_last_error", "sad_gated_scan_workspace_bytes", "sad_gated_scan_kept_bytes", "sad_gated_scan_codes_bytes",
+             "sad_gated_scan_fwd", "sad_gated_scan_bwd", "sad_gated_scan_step", "sad_checkpoint8_bytes", "sad_checkpoint8_save",
+             "sad_checkpoint8_restore", "sad_weight_grad8_workspace_bytes", "sad_weight_grad8")
+    good = [ctypes.cast(getattr(l, n), ctypes.c_void_p).value for n in names]
+    ops.bind(good)
+    for i in range(12):
+        for other in (0, 16, good[(i + 1) % 12], good[i] + 1, ctypes.cast(ctypes.CDLL(None).abort, ctypes.c_void_p).value):
+            with pytest.raises(RuntimeError, match="address %d is not %s" % (i, names[i])):
+                ops.bind(good[:i] + [other] + good[i + 1:])
+    # what was bound stays
+    with pytest.raises(RuntimeError, match="holds 34 bytes"):
+        ops.restore8(torch.zeros(1, dtype=torch.uint8), [1, 5], F32)
