@@ -3,8 +3,8 @@
 //   dW[n][k] = sum_m dY[m][n] X^[m][k] ,   db[n] = sum_m dY[m][n]           (m: token rows, the reduced index)
 //
 // X^ is decoded on its way into LDS; its values are exact in bf16 and fp16 (ckpt8.hpp), so the products are those of dY
-// with the checkpoint and nothing is rounded but the fp32 sums.  dY in float32 is split into three bf16 parts
-// (8 + 8 + 8 significant bits, exact), one matrix instruction each.  The workgroups of the first k
+// with the checkpoint and nothing is rounded but the fp32 sums.  dY in float32 is cut into three bf16 parts
+// (8 + 8 + 8 significant bits, exact; infinities and the largest floats stay what they are), one matrix instruction each.  The workgroups of the first k
 // tile also add up the columns of dY that pass through their registers: db.
 //
 // Both operands are stored with the reduced index slow, so fragments are read from LDS with the transposing read
@@ -65,7 +65,7 @@ template <> struct DyChunk<SAD_SRC_F32> { f32x4 a, b; };
 
 __device__ __forceinline__ unsigned c8_pack16(float a, float b, bool half) {
     if (half) return (unsigned)__builtin_bit_cast(unsigned short, (_Float16)a) | ((unsigned)__builtin_bit_cast(unsigned short, (_Float16)b) << 16);
-    // exact in bf16: the upper halves
+    // the upper halves (bf16 values are exact in them)
     return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
 }
 
@@ -200,9 +200,14 @@ template <class W, bool BIAS> struct Wgrad8 {
                 u32x4 v;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    v[j] = pack_bf16x2(rest[2 * j], rest[2 * j + 1]);
-                    rest[2 * j] -= __builtin_bit_cast(float, v[j] << 16);
-                    rest[2 * j + 1] -= __builtin_bit_cast(float, v[j] & 0xffff0000u);
+                    // cut, not rounded: the largest floats round to infinity in bf16
+                    v[j] = c8_pack16(rest[2 * j], rest[2 * j + 1], false);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float r = rest[2 * j + h], part = __builtin_bit_cast(float, __builtin_bit_cast(unsigned, r) & 0xffff0000u);
+                        // nothing is left of an infinity; a NaN, whose upper half may read as one, leaves a NaN
+                        rest[2 * j + h] = q == 0 && __builtin_fabsf(r) == __builtin_inff() ? 0.f : r - part;
+                    }
                 }
                 *(u32x4*)(at + q * W::ABYTES) = v;
             }

@@ -234,3 +234,40 @@ def test_operators_check_their_own_arguments():
     ):
         with pytest.raises(RuntimeError, match=message):
             call()
+
+
+def _f32(bits):
+    import struct
+    return struct.unpack("f", struct.pack("I", bits))[0]
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 21, 50), (700, 130, 33), (4100, 40, 40)])
+@pytest.mark.parametrize("value", [0x7f800000, 0xff800000, 0x7f7fffff, 0xff7fffff, 0x7f7f8000, 0x7f7f7fff, 0x7f800001, 0x7fc00000],
+                         ids=["inf", "-inf", "max", "-max", "rounds up in bf16", "rounds down in bf16", "NaN in the low half", "NaN"])
+def test_weight_grad_of_float32_at_the_end_of_the_range(M, N, K, value):
+    """dY as float32 enters in parts: an infinity stays one, a largest finite entry stays finite, and other rows of dW keep their
+    bits.  Tolerance: three exact products of M terms each, added in float32: 3 M 2^-24 sum|terms|."""
+    import numpy as np
+    torch, Fn = _t()
+    torch.manual_seed(M)
+    x = torch.randn(M, K, device="cuda") * 2.0 ** -12
+    x[M // 2, 3] = 0.0
+    dy = torch.randn(M, N, device="cuda")
+    ck = Fn.checkpoint8(x)
+    dw, db = Fn.weight_grad8(dy, ck, bias=True)
+    big = dy.clone()
+    big[:, 5] = 0.0
+    big.view(torch.int32)[M // 2, 5] = value - (1 << 32 if value >> 31 else 0)
+    gw, gb = Fn.weight_grad8(big, ck, bias=True)
+    v = _f32(value)
+    xv = ck.restore().double().cpu().numpy()
+    with np.errstate(all="ignore"):
+        want = np.float64(v) * xv[M // 2] + (0.0 * xv).sum(0)
+        got = gw[5].double().cpu().numpy()
+        if np.isfinite(v):
+            assert (np.abs(got - want) <= 3 * M * 2.0 ** -24 * np.abs(want)).all()
+        else:
+            assert np.array_equal(got, want, equal_nan=True)
+    assert np.array_equal(gb[5].double().cpu().numpy(), np.float64(v), equal_nan=True)
+    rest = [n for n in range(N) if n != 5]
+    assert torch.equal(gw[rest], dw[rest]) and torch.equal(gb[rest], db[rest])
