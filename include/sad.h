@@ -352,7 +352,8 @@ int sad_soft_finalize(int32_t B, int32_t T, int32_t V, int32_t steps, int32_t ov
  * pre-activations of D channels (gated == 0: [x | f]), e.g. one linear layer's output:
  *     s_t = sigmoid(-f_t),  h_t = h_{t-1} + s_t (x_t - h_{t-1}),  y_t = sigmoid(o_t) h_t      for t < lengths[b]
  * in time order, or from t = lengths[b] - 1 down to 0 (reverse).  y is 0 and the state unchanged at t >= lengths[b];
- * such rows of z and dy are not used, and dz is 0 there.  State and sums are fp32.
+ * such rows of z and dy are not used, and dz is 0 there.  State and sums are fp32; infinities are those of (1 - s) h + s x (an
+ * infinite state stays infinite past finite tokens).
  * The last axis of z, y, dy, dz has unit stride; rows are addressed through element strides; h0, h_last, dh_last, dh0 are
  * dense [B,D]. */
 typedef struct sad_scan_args {

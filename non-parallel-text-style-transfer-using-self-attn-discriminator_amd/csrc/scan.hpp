@@ -109,6 +109,15 @@ __device__ __forceinline__ float sc_share(float f) { return __builtin_amdgcn_rcp
 // 1 / (1 + u) = sigmoid(-f) and u / (1 + u) = sigmoid(f), each at full relative precision.
 __device__ __forceinline__ float sc_odds(float arg) { return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(arg, 126.0f)); }
 
+// The part of a state (or of a carried gradient) that an update takes away from it, h - s h: an infinite one loses a finite
+// amount and stays infinite, as in (1 - s) h; a NaN is one through the h that the update adds to.  One instruction in
+// the chain of steps ([4, 8191, 512] fp16: 38.9 us with it, 38.0 without).  Computing a block again where a state turned
+// NaN costs nothing otherwise, but the second form of the block rounds other channels' fp16 results differently.
+__device__ __forceinline__ float sc_lose(float h) {
+    constexpr float top = 3.402823466e38f;      // the largest float
+    return __builtin_amdgcn_fmed3f(h, -top, top);
+}
+
 // position of a wave
 struct ScanAt {
     int b, cg, ord, cc, len, lo, hi;      // ord: chunk in the order of the walk; [lo, hi) its blocks
@@ -154,7 +163,7 @@ __device__ __forceinline__ ScanAt scan_at(const ScanP& p, bool backward) {
 
 __device__ __forceinline__ void scan_apply(f32x2& h, f32x2 m, f32x2 v) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) h[e] = __builtin_fmaf(-m[e], h[e], h[e]) + v[e];
+    for (int e = 0; e < 2; ++e) h[e] = __builtin_fmaf(-m[e], sc_lose(h[e]), h[e]) + v[e];
 }
 
 // The state that enters a chunk: the maps of the groups in front of its group, then of its predecessors in the group.
@@ -408,7 +417,7 @@ __global__ __launch_bounds__(256) void k_scan_fwd(ScanP p) {
                 const f32x2 xv = Pair<KIND>::get(z[0][i]), fv = Pair<KIND>::get(z[1][i]);
                 f32x2 hn;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) hn[e] = __builtin_fmaf(sc_share(fv[e]), xv[e] - h[e], h[e]);
+                for (int e = 0; e < 2; ++e) hn[e] = __builtin_fmaf(sc_share(fv[e]), xv[e] - sc_lose(h[e]), h[e]);
                 h = sc_select(ok, hn, h);
                 f32x2 yv = h;
                 if constexpr (GATED) {
@@ -453,7 +462,7 @@ __global__ __launch_bounds__(64 * SC_GROUP) void k_scan_sum(ScanP p) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float s = sc_share(fv[e]);
-                h[e] = ok ? __builtin_fmaf(s, xv[e] - h[e], h[e]) : h[e];
+                h[e] = ok ? __builtin_fmaf(s, xv[e] - sc_lose(h[e]), h[e]) : h[e];
                 m[e] = ok ? __builtin_fmaf(s, 1.0f - m[e], m[e]) : m[e];
             }
         }
@@ -594,7 +603,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanP p) {
             static_for<SC_STEPS>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const int t = kb * SC_STEPS + (p.reverse ? SC_STEPS - 1 - i : i);
-                const f32x2 fa = in.template times<1, i, MODE == SC_EDGE>(SC_LOG2E), xd = in.template x_less<i, MODE == SC_EDGE>(hc);
+                const f32x2 fa = in.template times<1, i, MODE == SC_EDGE>(SC_LOG2E), xd = in.template x_less<i, MODE == SC_EDGE>(f32x2{sc_lose(hc[0]), sc_lose(hc[1])});
                 f32x2 hn;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -630,7 +639,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_bwd(ScanP p) {
                     const float g = dh + carry[e], sv = __builtin_amdgcn_rcpf(1.0f + odds[i][e]);
                     dx[e] = sv * g;
                     df[e] = -(odds[i][e] * sv * dx[e]) * xd[e];
-                    cn[e] = __builtin_fmaf(-sv, g, g);
+                    cn[e] = __builtin_fmaf(-sv, sc_lose(g), g);
                 }
                 const f32x2 none{0.f, 0.f};
                 carry = sc_select(ok, cn, carry);
@@ -699,7 +708,7 @@ __global__ __launch_bounds__(64 * SC_GROUP) void k_scan_bsum(ScanP p) {
                     float dh = dyv[e];
                     if constexpr (GATED) dh *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(oa[e]));
                     const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(fa[e])), g = dh + v[e];
-                    v[e] = ok ? __builtin_fmaf(-s, g, g) : v[e];
+                    v[e] = ok ? __builtin_fmaf(-s, sc_lose(g), g) : v[e];
                     m[e] = ok ? __builtin_fmaf(s, 1.0f - m[e], m[e]) : m[e];
                 }
             });
@@ -723,7 +732,7 @@ __global__ __launch_bounds__(256) void k_scan_step(int D, int per, const void* _
     const long long zo = (long long)b * z_sb + c;
     const float hp = h[(long long)b * h_sb + c];
     const float x = Elem<KIND>::load(z, zo), f = Elem<KIND>::load(z, zo + D);
-    float hn = __builtin_fmaf(sc_share(f), x - hp, hp), yv = hn;
+    float hn = __builtin_fmaf(sc_share(f), x - sc_lose(hp), hp), yv = hn;
     if constexpr (GATED) yv *= sigmoidf_(Elem<KIND>::load(z, zo + 2ll * D));
     const bool live = alive == nullptr || alive[b] != 0;
     Elem<KIND>::store(y, (long long)b * y_sb + c, live ? yv : 0.f);

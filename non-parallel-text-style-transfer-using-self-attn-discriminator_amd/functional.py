@@ -738,7 +738,8 @@ def gated_scan(z, h0=None, lengths=None, reverse=False, gated_output=True, save=
     y = h), float32 / bfloat16 / float16, any batch and time strides with unit channel stride (the output of one linear
     layer; time-major storage as a transposed view); y and the gradient come back in the same type and axis order.
     ``h0`` [B,D] float32 is the state in front of the first token (default 0), ``h_last`` float32 the one after the last: a
-    long text can be read in pieces.  ``lengths`` [B] (host or device, 0..T, any order): y is 0 at t >= length, the state
+    long text can be read in pieces.  A NaN or an infinity stays in its channel; an infinite state is infinite until an opposite one
+    makes it NaN.  ``lengths`` [B] (host or device, 0..T, any order): y is 0 at t >= length, the state
     stays, and such rows of z may hold anything.  ``reverse`` runs from the last token to the first.
 
     Differentiable in z and h0, once and in reverse mode (dual tensors are refused).  ``save="input"`` keeps z for the backward pass; ``save="int8"`` keeps its 8-bit codes
