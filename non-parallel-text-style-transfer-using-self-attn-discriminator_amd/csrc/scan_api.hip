@@ -63,7 +63,8 @@ int scan_chunks(int B, int T, int D) {
 int check_scan_dims(int B, int T, int D, int kind) {
     if (B < 1 || T < 1 || D < 2) return set_error(-1, "gated scan needs B >= 1, T >= 1, D >= 2 (B=%d T=%d D=%d)", B, T, D);
     if (D > (1 << 24) || T > (1 << 28)) return set_error(-1, "gated scan: D=%d or T=%d beyond the supported maximum", D, T);
-    if ((long long)B * ceil_div(D, SC_CH) * 64 > MAX_GRID) return set_error(-1, "gated scan: B=%d x D=%d beyond the supported maximum", B, D);
+    // one wave per sentence and 128 channels (more only where there are few): a launch holds fewer than 2^32 threads
+    if (((long long)B * ceil_div(D, SC_CH) + 3) / 4 * 256 > 0xffffffffll) return set_error(-1, "gated scan: B=%d x D=%d beyond the supported maximum", B, D);
     if (!known_kind(kind)) return set_error(-1, "kind must be SAD_SRC_F32, SAD_SRC_BF16 or SAD_SRC_F16, got %d", kind);
     return 0;
 }

@@ -271,3 +271,19 @@ def test_weight_grad_of_float32_at_the_end_of_the_range(M, N, K, value):
     assert np.array_equal(gb[5].double().cpu().numpy(), np.float64(v), equal_nan=True)
     rest = [n for n in range(N) if n != 5]
     assert torch.equal(gw[rest], dw[rest]) and torch.equal(gb[rest], db[rest])
+
+
+def test_more_than_2_31_threads():
+    """A batch whose launch has more than 2^31 threads: forward and backward of its ends equal those of the ends alone."""
+    torch, Fn = _t()
+    B = 2 ** 25 + 100
+    g = torch.Generator(device="cuda").manual_seed(1)
+    z = torch.empty(B, 1, 6, dtype=torch.float16, device="cuda").normal_(generator=g).requires_grad_(True)
+    dy = torch.empty(B, 1, 2, dtype=torch.float16, device="cuda").normal_(generator=g)
+    y, last = Fn.gated_scan(z)
+    dz, = torch.autograd.grad([y, last], z, [dy, torch.ones_like(last)])
+    for rows in (slice(0, 64), slice(B // 2, B // 2 + 64), slice(B - 64, B)):
+        zz = z.detach()[rows].clone().requires_grad_(True)
+        yy, ll = Fn.gated_scan(zz)
+        assert torch.equal(y[rows], yy) and torch.equal(last[rows], ll)
+        assert torch.equal(dz[rows], torch.autograd.grad([yy, ll], zz, [dy[rows], torch.ones_like(ll)])[0])

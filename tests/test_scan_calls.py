@@ -145,3 +145,13 @@ def test_bind_takes_the_library_s_own_functions_only():
     # what was bound stays
     with pytest.raises(RuntimeError, match="holds 34 bytes"):
         ops.restore8(torch.zeros(1, dtype=torch.uint8), [1, 5], F32)
+
+
+def test_size_limits_are_those_of_a_launch():
+    l = lib.load()
+    most = (2 ** 32 - 1) // 64 // 4 * 4                          # waves of 64 threads in workgroups of four
+    for B, D in ((most, 2), (most, 128), (most // 2, 129), (1, 1 << 24), (2 ** 25 + 100, 2)):
+        assert l.sad_gated_scan_workspace_bytes(B, 1, D) == 16, (B, D)
+        assert l.sad_gated_scan_kept_bytes(B, 1, D) == B * D * 4
+    for B, D in ((most + 1, 2), (most // 2 + 1, 129), (2 ** 31 - 1, 2)):
+        assert l.sad_gated_scan_workspace_bytes(B, 1, D) == 0 and "beyond the supported maximum" in lib.last_error()
