@@ -209,7 +209,11 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
                     "gated_scan: the lengths came back as another tensor");
         const c10::DeviceGuard guard(kept.device());
         const auto options = kept.options().dtype((at::ScalarType)v[6]);
-        Tensor dz = is_dense(size, stride) ? at::empty_strided(size, stride, options) : at::empty(size, options), dh0;
+        // in z's order: its strides, or those of its axes without the gaps
+        Tensor dz, dh0;
+        if (is_dense(size, stride)) dz = at::empty_strided(size, stride, options);
+        else if (size[0] > 1 && size[1] > 1 && stride[0] < stride[1]) dz = at::empty_strided(size, {size[2], size[0] * size[2], 1}, options);
+        else dz = at::empty(size, options);
         const ScanShape s = scan_shape(dz, gated);
         if (dy.defined() && dy.stride(2) != 1) dy = dy.contiguous();
         if (dh.defined()) dh = dh.contiguous();

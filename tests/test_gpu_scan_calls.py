@@ -287,3 +287,22 @@ def test_more_than_2_31_threads():
         yy, ll = Fn.gated_scan(zz)
         assert torch.equal(y[rows], yy) and torch.equal(last[rows], ll)
         assert torch.equal(dz[rows], torch.autograd.grad([yy, ll], zz, [dy[rows], torch.ones_like(ll)])[0])
+
+
+@pytest.mark.parametrize("save", ["input", "int8"])
+def test_gradient_of_time_major_rows_of_a_wider_matrix(save):
+    """y and dz come back in z's axis order, also where z's rows have gaps."""
+    torch, Fn = _t()
+    torch.manual_seed(12)
+    T, B, D = 21, 5, 12
+    wide = torch.randn(T, B, 3 * D + 7, device="cuda")
+    got = []
+    for z in (wide[..., 2:2 + 3 * D].transpose(0, 1), wide[..., 2:2 + 3 * D].transpose(0, 1).contiguous()):
+        z = z.detach().requires_grad_(True)
+        y, last = Fn.gated_scan(z, save=save)
+        grads = []
+        z.register_hook(lambda g: grads.append(g))
+        (y.square().sum() + last.sum()).backward()
+        got.append((y, grads[0]))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and a.transpose(0, 1).is_contiguous() and b.is_contiguous()
