@@ -71,6 +71,7 @@ void bind(at::IntArrayRef a) {
     api = next;
 }
 
+void need_bound() { TORCH_CHECK(api.last_error != nullptr, "torch.ops.sad_amd is not bound to libsad: use sad_amd.functional"); }
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, "libsad ", what, " failed (", rc, "): ", api.last_error()); }
 size_t size_of(size_t n, const char* what) {
     TORCH_CHECK(n != 0, "libsad ", what, " failed: ", api.last_error());
@@ -96,6 +97,7 @@ variable_list once(variable_list grads, const char* name) {
 // The kernels follow data pointers: every tensor has to have memory on the device.  Fake and meta tensors (tracing) and the
 // wrappers of function transforms have none.
 void need_memory(const Tensor& t, const char* name, const char* what) {
+    need_bound();
     TORCH_CHECK(t.has_storage() && t.storage().device_type() != at::kMeta, name, ": ", what,
                 " has no memory (a meta or fake tensor, or the wrapper of a function transform); the operator cannot be traced");
     TORCH_CHECK(t.is_cuda(), name, ": ", what, " must be on the HIP device, got ", t.device(), "; there is no CPU path");
@@ -306,6 +308,7 @@ Tensor checkpoint8(const Tensor& x) {
 
 // `saved` is the caller's to move, copy and slice: it has to be a whole checkpoint of rows x C entries, on the device
 void need_saved(const Tensor& saved, int64_t rows, int64_t C) {
+    need_bound();
     TORCH_CHECK(saved.scalar_type() == at::kByte && saved.is_contiguous(), "a checkpoint's codes are contiguous uint8, got ", saved.scalar_type(),
                 saved.is_contiguous() ? "" : " (not contiguous)");
     const size_t n = rows > 0 && C > 0 ? size_of(api.ckpt_bytes(rows, C), "sad_checkpoint8_bytes") : 0;

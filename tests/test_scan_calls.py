@@ -155,3 +155,26 @@ def test_size_limits_are_those_of_a_launch():
         assert l.sad_gated_scan_kept_bytes(B, 1, D) == B * D * 4
     for B, D in ((most + 1, 2), (most // 2 + 1, 129), (2 ** 31 - 1, 2)):
         assert l.sad_gated_scan_workspace_bytes(B, 1, D) == 0 and "beyond the supported maximum" in lib.last_error()
+
+
+def test_operators_without_the_library_raise():
+    """The operator library loaded by itself has no functions to call: every operator says so instead of following NULL."""
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+torch.ops.load_library(sys.argv[1])
+o, f, u = torch.ops.sad_amd, torch.zeros, torch.zeros(102, dtype=torch.uint8)
+for call in (lambda: o.gated_scan(f(2, 3, 12), None, None, False, True, False), lambda: o.gated_scan_step(f(2, 12), f(2, 4), None, True, f(2, 4)),
+             lambda: o.checkpoint8(f(3, 5)), lambda: o.restore8(u, [3, 5], torch.float32), lambda: o.weight_grad8(f(3, 2), u, 5, True),
+             lambda: o.linear8(f(3, 5), f(2, 5), None)):
+    try:
+        call()
+    except RuntimeError as e:
+        assert "not bound" in str(e), e
+    else:
+        raise AssertionError("no error")
+print("done")
+"""
+    r = subprocess.run([sys.executable, "-c", code, lib.OPS_PATH], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split()[-1] == "done", (r.returncode, r.stderr[-400:])
