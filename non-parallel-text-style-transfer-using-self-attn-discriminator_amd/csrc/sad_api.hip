@@ -27,14 +27,6 @@ namespace {
 
 thread_local char g_err[512] = "";
 
-int fail(int code, const char* fmt, ...) {
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_err, sizeof(g_err), fmt, ap);
-    va_end(ap);
-    return code;
-}
-
 }  // namespace
 
 namespace sad {
@@ -54,7 +46,7 @@ namespace {
 #define SAD_CHECK_LAUNCH(name)                                                          \
     do {                                                                                \
         hipError_t e__ = hipGetLastError();                                             \
-        if (e__ != hipSuccess) return fail(-2, "%s: %s", name, hipGetErrorString(e__)); \
+        if (e__ != hipSuccess) return set_error(-2, "%s: %s", name, hipGetErrorString(e__)); \
     } while (0)
 
 size_t align_up(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -244,15 +236,15 @@ WsLayout ws_layout(const Shape& s) {
 }
 
 int check_dims(const sad_dims* d, Shape* s) {
-    if (d == nullptr) return fail(-1, "dims is NULL");
+    if (d == nullptr) return set_error(-1, "dims is NULL");
     if (d->B < 1 || d->T < 1 || d->V < 1 || d->E < 1 || d->H < 1 || d->L < 1)
-        return fail(-1, "dims must be positive (B=%d T=%d V=%d E=%d H=%d L=%d)", d->B, d->T, d->V, d->E, d->H, d->L);
-    if (d->T > ATT_MAX_T) return fail(-1, "T=%d exceeds the supported maximum %d", d->T, ATT_MAX_T);
-    if (d->L > ATT_MAX_L) return fail(-1, "L=%d exceeds the supported maximum %d", d->L, ATT_MAX_L);
-    if (d->H > 2048) return fail(-1, "H=%d exceeds the supported maximum 2048", d->H);
-    if ((long long)d->B * d->T > (1ll << 30)) return fail(-1, "B*T too large");
-    if (d->B > 65535 * 64) return fail(-1, "B too large");
-    if (d->cell != SAD_CELL_LSTM && d->cell != SAD_CELL_GRU) return fail(-1, "cell=%d is neither SAD_CELL_LSTM nor SAD_CELL_GRU", d->cell);
+        return set_error(-1, "dims must be positive (B=%d T=%d V=%d E=%d H=%d L=%d)", d->B, d->T, d->V, d->E, d->H, d->L);
+    if (d->T > ATT_MAX_T) return set_error(-1, "T=%d exceeds the supported maximum %d", d->T, ATT_MAX_T);
+    if (d->L > ATT_MAX_L) return set_error(-1, "L=%d exceeds the supported maximum %d", d->L, ATT_MAX_L);
+    if (d->H > 2048) return set_error(-1, "H=%d exceeds the supported maximum 2048", d->H);
+    if ((long long)d->B * d->T > (1ll << 30)) return set_error(-1, "B*T too large");
+    if (d->B > 65535 * 64) return set_error(-1, "B too large");
+    if (d->cell != SAD_CELL_LSTM && d->cell != SAD_CELL_GRU) return set_error(-1, "cell=%d is neither SAD_CELL_LSTM nor SAD_CELL_GRU", d->cell);
     *s = make_shape(d->B, d->T, d->V, d->E, d->H, d->L, d->cell);
     return 0;
 }
@@ -263,11 +255,11 @@ template <class T>
 const T* at(const void* base, size_t off) { return (const T*)((const char*)base + off); }
 
 int check_ptr(const void* p, const char* name) {
-    if (p == nullptr) return fail(-1, "%s is NULL", name);
+    if (p == nullptr) return set_error(-1, "%s is NULL", name);
     return 0;
 }
 int check_aligned(const void* p, size_t a, const char* name) {
-    if (((uintptr_t)p) % a) return fail(-1, "%s must be %zu-byte aligned", name, a);
+    if (((uintptr_t)p) % a) return set_error(-1, "%s must be %zu-byte aligned", name, a);
     return 0;
 }
 
@@ -321,7 +313,7 @@ int run_softemb_fwd(const Shape& s, const PackedLayout& pl, const WsLayout& wl, 
     bf16raw* X = at<bf16raw>(ws, wl.off[SAD_WS_X]);
     float* accf = at<float>(ws, wl.off[SAD_WS_ACCF]);
     if (kind != SAD_SRC_F32 && kind != SAD_SRC_BF16)
-        return fail(-1, "soft-embedding stage needs SAD_SRC_F32 or SAD_SRC_BF16, got %d", kind);
+        return set_error(-1, "soft-embedding stage needs SAD_SRC_F32 or SAD_SRC_BF16, got %d", kind);
     if (check_aligned(src, kind == SAD_SRC_F32 ? 4 : 2, "src")) return -1;
     if (s.Ep == 320 && s.V >= 64) {
         // The shipped embedding size (E = 289..320): stream-K over the non-empty 128-row tiles, one
@@ -364,7 +356,7 @@ int run_softemb_bwd(const Shape& s, const PackedLayout& pl, const WsLayout& wl, 
     const bf16raw* wemb = at<bf16raw>(packed, pl.wemb);
     const bf16raw* DX = at<bf16raw>(ws, wl.off[SAD_WS_DX]);
     if (kind != SAD_SRC_F32 && kind != SAD_SRC_BF16)
-        return fail(-1, "d(soft tokens) needs SAD_SRC_F32 or SAD_SRC_BF16, got %d", kind);
+        return set_error(-1, "d(soft tokens) needs SAD_SRC_F32 or SAD_SRC_BF16, got %d", kind);
     if (check_aligned(dsrc, kind == SAD_SRC_F32 ? 4 : 2, "dsrc")) return -1;
     if (s.Ep == 320) {
         // A-stationary fast path for the shipped embedding size (E = 289..320 -> Ep = 320 = 32*10).
@@ -550,7 +542,7 @@ size_t sad_workspace_bytes(const sad_dims* d) {
 int sad_workspace_field(const sad_dims* d, int field, size_t* offset, size_t* bytes) {
     Shape s;
     if (check_dims(d, &s)) return -1;
-    if (field < 0 || field >= SAD_WS_NFIELDS) return fail(-1, "unknown workspace field %d", field);
+    if (field < 0 || field >= SAD_WS_NFIELDS) return set_error(-1, "unknown workspace field %d", field);
     WsLayout w = ws_layout(s);
     if (offset) *offset = w.off[field];
     if (bytes) *bytes = w.bytes[field];
@@ -567,7 +559,7 @@ int sad_pack_weights(const sad_dims* d, const sad_weights* w, void* packed, void
                           w->linear_emb_bias, w->linear_q_weight, w->linear_q_bias, w->linear_attn_weight,
                           w->linear_attn_bias, w->output_layer_weight, w->output_layer_bias};
     for (size_t i = 0; i < sizeof(need) / sizeof(need[0]); ++i)
-        if (need[i] == nullptr) return fail(-1, "sad_weights field #%zu is NULL", i);
+        if (need[i] == nullptr) return set_error(-1, "sad_weights field #%zu is NULL", i);
     hipStream_t st = (hipStream_t)stream;
     ensure_hostflag();                                       // set-up call: the time-out word of this device
     const PackedLayout p = packed_layout(s);
@@ -910,7 +902,7 @@ int run_zero_sync(const Ctx& c, bool with_timeout_words) {
     const size_t counters = (size_t)lp_err_line(c.s.B) * LP_SYNC_PITCH * 4;
     const size_t n = with_timeout_words ? c.wl.bytes[SAD_WS_SYNC] : counters;
     if (hipMemsetAsync(at<unsigned char>(c.ws, c.wl.off[SAD_WS_SYNC]), 0, n, c.st) != hipSuccess)
-        return fail(-2, "hipMemsetAsync(SYNC) failed");
+        return set_error(-2, "hipMemsetAsync(SYNC) failed");
     return 0;
 }
 
@@ -936,7 +928,7 @@ int noalloc_scratch(unsigned char** out) {
         void* p = nullptr;
         const hipError_t e = hipGetSymbolAddress(&p, HIP_SYMBOL(g_noalloc_scratch));
         if (e != hipSuccess || p == nullptr)
-            return fail(-2, "hipGetSymbolAddress(scratch) failed on device %d: %s", dev, hipGetErrorString(e));
+            return set_error(-2, "hipGetSymbolAddress(scratch) failed on device %d: %s", dev, hipGetErrorString(e));
         g_noalloc_ptr[dev] = (unsigned char*)p;
     }
     *out = g_noalloc_ptr[dev];
@@ -945,8 +937,8 @@ int noalloc_scratch(unsigned char** out) {
 
 // Context of RNN layer i above the first: dims {B, T, 1, 2H, H, L, cell}, the caller's image and workspace.
 int make_upper_ctx(const Ctx& c0, const sad_rnn_layer* upper, int n_upper, int i, Ctx* cu) {
-    if (n_upper < 0 || n_upper > SAD_MAX_UPPER_LAYERS) return fail(-1, "n_upper=%d outside 0..%d", n_upper, SAD_MAX_UPPER_LAYERS);
-    if (upper == nullptr) return fail(-1, "n_upper=%d but upper is NULL", n_upper);
+    if (n_upper < 0 || n_upper > SAD_MAX_UPPER_LAYERS) return set_error(-1, "n_upper=%d outside 0..%d", n_upper, SAD_MAX_UPPER_LAYERS);
+    if (upper == nullptr) return set_error(-1, "n_upper=%d but upper is NULL", n_upper);
     sad_dims du = {c0.s.B, c0.s.T, 1, 2 * c0.s.H, c0.s.H, c0.s.L, c0.s.cell};
     if (make_ctx(&du, upper[i].packed, upper[i].workspace, (void*)c0.st, cu)) return -1;
     cu->upper = true;
@@ -979,8 +971,8 @@ int run_upper_fwd(const Ctx& c0, const sad_fwd_args* a) {
 }
 
 int check_upper(const sad_rnn_layer* upper, int n_upper) {
-    if (n_upper < 0 || n_upper > SAD_MAX_UPPER_LAYERS) return fail(-1, "n_upper=%d outside 0..%d", n_upper, SAD_MAX_UPPER_LAYERS);
-    if (n_upper > 0 && upper == nullptr) return fail(-1, "n_upper=%d but upper is NULL", n_upper);
+    if (n_upper < 0 || n_upper > SAD_MAX_UPPER_LAYERS) return set_error(-1, "n_upper=%d outside 0..%d", n_upper, SAD_MAX_UPPER_LAYERS);
+    if (n_upper > 0 && upper == nullptr) return set_error(-1, "n_upper=%d but upper is NULL", n_upper);
     return 0;
 }
 
@@ -990,14 +982,14 @@ int forward_impl(const Ctx& c_in, const sad_fwd_args* a) {
     const Ctx& c = c_in;
     const Shape& s = c.s;
     if (const unsigned code = take_hostflag())
-        return fail(-4, "a hand-off wait inside the persistent %s of an EARLIER call on this device timed out (its workgroups "
+        return set_error(-4, "a hand-off wait inside the persistent %s of an EARLIER call on this device timed out (its workgroups "
                         "were not co-resident: another kernel on the device?); logits / loss / d(soft tokens) of that call "
                         "are NaN.  This call was not started; the next one will be",
                     code == 2 ? "BPTT" : "forward recurrence");
     if (check_ptr(a->src, "src") || check_ptr(a->lengths, "lengths") || check_ptr(a->mask, "mask") ||
         check_ptr(a->logits, "logits") || check_ptr(a->weights, "weights"))
         return -1;
-    if (a->loss != nullptr && a->labels == nullptr) return fail(-1, "loss requested without labels");
+    if (a->loss != nullptr && a->labels == nullptr) return set_error(-1, "loss requested without labels");
     bf16raw* X = at<bf16raw>(c.ws, c.wl.off[SAD_WS_X]);
     // need bits, row lists, tile list (the same launch zeroes the hand-off counters and timeout words of the recurrence)
     int rc = run_prep(s, c.wl, c.ws, a->lengths, a->mask, a->mask_stride_b, a->mask_stride_t, a->guard, c.st);
@@ -1014,7 +1006,7 @@ int forward_impl(const Ctx& c_in, const sad_fwd_args* a) {
     } else if (a->onehot_ids != nullptr) {
         // one-hot soft tokens with their (index, value) side channel: K1 forward is a scaled gather
         if (a->src_kind != SAD_SRC_F32 && a->src_kind != SAD_SRC_BF16)
-            return fail(-1, "soft tokens need SAD_SRC_F32 or SAD_SRC_BF16, got %d", a->src_kind);
+            return set_error(-1, "soft tokens need SAD_SRC_F32 or SAD_SRC_BF16, got %d", a->src_kind);
         if (check_ptr(a->onehot_val, "onehot_val") || check_aligned(a->onehot_ids, 8, "onehot_ids")) return -1;
         const long long chunks = (long long)s.M * (s.Ep / 8);
         int blocks = (int)((chunks + 255) / 256);
@@ -1038,7 +1030,7 @@ int forward_impl(const Ctx& c_in, const sad_fwd_args* a) {
 int check_bwd_args(const sad_bwd_args* a) {
     if (check_ptr(a, "args")) return -1;
     if (check_ptr(a->weights, "weights") || check_ptr(a->logits, "logits")) return -1;
-    if (a->dlogits == nullptr && a->labels == nullptr) return fail(-1, "need dlogits, or labels (+ dloss / dloss_scale)");
+    if (a->dlogits == nullptr && a->labels == nullptr) return set_error(-1, "need dlogits, or labels (+ dloss / dloss_scale)");
     return 0;
 }
 
@@ -1074,9 +1066,9 @@ int sad_backward(const sad_dims* d, const void* packed, const sad_bwd_args* a, v
             const Ctx& u = cu[i];
             // the key columns of this layer's dZ have no producer (no attention on upper layers): all zero
             if (hipMemsetAsync(at<unsigned char>(u.ws, u.wl.off[SAD_WS_DZ]), 0, u.wl.bytes[SAD_WS_DZ], u.st) != hipSuccess)
-                return fail(-2, "hipMemsetAsync(DZ) failed");
+                return set_error(-2, "hipMemsetAsync(DZ) failed");
             if (i != top && hipMemsetAsync(at<unsigned char>(u.ws, u.wl.off[SAD_WS_DHFIN]), 0, u.wl.bytes[SAD_WS_DHFIN], u.st) != hipSuccess)
-                return fail(-2, "hipMemsetAsync(DHFIN) failed");
+                return set_error(-2, "hipMemsetAsync(DHFIN) failed");
             if ((rc = run_zero_sync(u, false)) != 0) return rc;      // hand-off counters of this layer's BPTT
             if ((rc = run_lstm_bwd(u, dhs, u.s.Ep)) != 0) return rc;
             if ((rc = run_inproj_bwd(u)) != 0) return rc;
@@ -1086,7 +1078,7 @@ int sad_backward(const sad_dims* d, const void* packed, const sad_bwd_args* a, v
             dhs = at<bf16raw>(u.ws, u.wl.off[SAD_WS_DX]);
         }
         if (hipMemsetAsync(at<unsigned char>(c.ws, c.wl.off[SAD_WS_DHFIN]), 0, c.wl.bytes[SAD_WS_DHFIN], c.st) != hipSuccess)
-            return fail(-2, "hipMemsetAsync(DHFIN) failed");
+            return set_error(-2, "hipMemsetAsync(DHFIN) failed");
         if ((rc = run_lstm_bwd(c, dhs, cu[0].s.Ep)) != 0) return rc;
     }
     if ((rc = run_inproj_bwd(c)) != 0) return rc;
@@ -1105,7 +1097,7 @@ int sad_forward_noalloc(const sad_dims* d, const void* packed, const sad_fwd_arg
     if (check_dims(d, &s)) return -1;
     const size_t need = ws_layout(s).total;
     if (need > (size_t)SAD_NOALLOC_MAX_BYTES)
-        return fail(-3, "sad_forward_noalloc: B=%d T=%d V=%d E=%d H=%d needs a workspace of %zu bytes, the static scratch "
+        return set_error(-3, "sad_forward_noalloc: B=%d T=%d V=%d E=%d H=%d needs a workspace of %zu bytes, the static scratch "
                         "holds %zu (use sad_forward with a caller-provided workspace)",
                     d->B, d->T, d->V, d->E, d->H, need, (size_t)SAD_NOALLOC_MAX_BYTES);
     unsigned char* scratch = nullptr;
@@ -1147,7 +1139,7 @@ int sad_attnpool_fwd(const sad_dims* d, const void* packed, const int64_t* label
     Ctx c;
     if (make_ctx(d, packed, ws, stream, &c)) return -1;
     if (check_ptr(logits, "logits") || check_ptr(weights, "weights")) return -1;
-    if (loss != nullptr && labels == nullptr) return fail(-1, "loss requested without labels");
+    if (loss != nullptr && labels == nullptr) return set_error(-1, "loss requested without labels");
     return run_attn_fwd(c, labels, logits, weights, loss);
 }
 
@@ -1160,11 +1152,11 @@ int sad_attnpool_bwd(const sad_dims* d, const void* packed, const sad_bwd_args* 
 
 int sad_gumbel_st_step(const sad_gumbel_args* a, void* stream) {
     if (check_ptr(a, "args")) return -1;
-    if (a->B < 1 || a->V < 1) return fail(-1, "B and V must be positive (B=%d V=%d)", a->B, a->V);
+    if (a->B < 1 || a->V < 1) return set_error(-1, "B and V must be positive (B=%d V=%d)", a->B, a->V);
     if (check_ptr(a->logits, "logits") || check_ptr(a->noise, "noise") || check_ptr(a->s_row, "s_row") ||
         check_ptr(a->idx, "idx") || check_ptr(a->val, "val"))
         return -1;
-    if (!(a->tau > 0.f)) return fail(-1, "tau must be positive");
+    if (!(a->tau > 0.f)) return set_error(-1, "tau must be positive");
     hipStream_t st = (hipStream_t)stream;
 #define SAD_GUMBEL(KIND)                                                                                              \
     hipLaunchKernelGGL((k_gumbel_st_fwd<KIND>), dim3(a->B), dim3(256), 0, st, a->B, a->V, a->logits,                   \
@@ -1173,7 +1165,7 @@ int sad_gumbel_st_step(const sad_gumbel_args* a, void* stream) {
                        a->alive_out)
     if (a->s_kind == SAD_SRC_F32) SAD_GUMBEL(SRC_F32);
     else if (a->s_kind == SAD_SRC_BF16) SAD_GUMBEL(SRC_BF16);
-    else return fail(-1, "s_kind must be SAD_SRC_F32 or SAD_SRC_BF16, got %d", a->s_kind);
+    else return set_error(-1, "s_kind must be SAD_SRC_F32 or SAD_SRC_BF16, got %d", a->s_kind);
 #undef SAD_GUMBEL
     SAD_CHECK_LAUNCH("k_gumbel_st_fwd");
     return 0;
@@ -1182,9 +1174,9 @@ int sad_gumbel_st_step(const sad_gumbel_args* a, void* stream) {
 int sad_gumbel_st_step_bwd(int32_t B, int32_t V, const void* d_s_row, int32_t s_kind, int64_t s_stride_b,
                            const float* d_rnn_in, const uint8_t* alive, const float* y_soft, float tau, float* dlogits,
                            int64_t dlogits_stride, void* stream) {
-    if (B < 1 || V < 1) return fail(-1, "B and V must be positive (B=%d V=%d)", B, V);
+    if (B < 1 || V < 1) return set_error(-1, "B and V must be positive (B=%d V=%d)", B, V);
     if (check_ptr(y_soft, "y_soft") || check_ptr(dlogits, "dlogits")) return -1;
-    if (d_s_row == nullptr && d_rnn_in == nullptr) return fail(-1, "need d_s_row or d_rnn_in");
+    if (d_s_row == nullptr && d_rnn_in == nullptr) return set_error(-1, "need d_s_row or d_rnn_in");
     hipStream_t st = (hipStream_t)stream;
     if (s_kind == SAD_SRC_F32)
         hipLaunchKernelGGL((k_gumbel_st_bwd<SRC_F32>), dim3(B), dim3(256), 0, st, B, V, d_s_row, (long long)s_stride_b, d_rnn_in,
@@ -1192,7 +1184,7 @@ int sad_gumbel_st_step_bwd(int32_t B, int32_t V, const void* d_s_row, int32_t s_
     else if (s_kind == SAD_SRC_BF16)
         hipLaunchKernelGGL((k_gumbel_st_bwd<SRC_BF16>), dim3(B), dim3(256), 0, st, B, V, d_s_row, (long long)s_stride_b, d_rnn_in,
                            alive, y_soft, tau, dlogits, (long long)dlogits_stride);
-    else return fail(-1, "s_kind must be SAD_SRC_F32 or SAD_SRC_BF16, got %d", s_kind);
+    else return set_error(-1, "s_kind must be SAD_SRC_F32 or SAD_SRC_BF16, got %d", s_kind);
     SAD_CHECK_LAUNCH("k_gumbel_st_bwd");
     return 0;
 }
@@ -1200,9 +1192,9 @@ int sad_gumbel_st_step_bwd(int32_t B, int32_t V, const void* d_s_row, int32_t s_
 int sad_soft_finalize(int32_t B, int32_t T, int32_t V, int32_t steps, int32_t over_max, int32_t pad_id, int32_t sos_id,
                       int32_t eos_id, void* S, int32_t s_kind, int64_t sT, int64_t sB, int64_t* ids, float* val,
                       const int32_t* lens_steps, const uint8_t* alive, int32_t* lens_out, uint8_t* mask, void* stream) {
-    if (B < 1 || V < 1 || T < 1 || steps < 0) return fail(-1, "bad sizes (B=%d T=%d V=%d steps=%d)", B, T, V, steps);
-    if (T < steps + 1) return fail(-1, "T=%d is too small for %d steps + [sos]", T, steps);
-    if (B > 65535) return fail(-1, "B too large for this entry point");
+    if (B < 1 || V < 1 || T < 1 || steps < 0) return set_error(-1, "bad sizes (B=%d T=%d V=%d steps=%d)", B, T, V, steps);
+    if (T < steps + 1) return set_error(-1, "T=%d is too small for %d steps + [sos]", T, steps);
+    if (B > 65535) return set_error(-1, "B too large for this entry point");
     if (check_ptr(S, "S") || check_ptr(ids, "ids") || check_ptr(val, "val") || check_ptr(lens_steps, "lens_steps") ||
         check_ptr(alive, "alive") || check_ptr(lens_out, "lens_out") || check_ptr(mask, "mask"))
         return -1;
@@ -1213,7 +1205,7 @@ int sad_soft_finalize(int32_t B, int32_t T, int32_t V, int32_t steps, int32_t ov
     else if (s_kind == SAD_SRC_BF16)
         hipLaunchKernelGGL((k_soft_finalize<SRC_BF16>), dim3(T, B), dim3(256), 0, st, B, T, V, steps, over_max, pad_id, sos_id, eos_id, S,
                            (long long)sT, (long long)sB, (long long*)ids, val, lens_steps, alive, lens_out, mask);
-    else return fail(-1, "s_kind must be SAD_SRC_F32 or SAD_SRC_BF16, got %d", s_kind);
+    else return set_error(-1, "s_kind must be SAD_SRC_F32 or SAD_SRC_BF16, got %d", s_kind);
     SAD_CHECK_LAUNCH("k_soft_finalize");
     return 0;
 }
@@ -1226,7 +1218,7 @@ int sad_debug_set(int32_t key, int64_t value) {
         case SAD_DBG_WITHHOLD_BWD: g_withhold_bwd.store((int)value); return 0;
         case SAD_DBG_WITHHOLD_UPPER_ONLY: g_withhold_upper_only.store(value != 0 ? 1 : 0); return 0;
         case SAD_DBG_WGRAD_ATOMICS: g_wgrad_atomics.store(value != 0 ? 1 : 0); return 0;
-        default: return fail(-1, "unknown debug key %d", key);
+        default: return set_error(-1, "unknown debug key %d", key);
     }
 }
 
@@ -1342,7 +1334,7 @@ int sad_param_grads_accumulate(const sad_dims* d, const sad_param_grads* g, cons
                                  g->embedding_weight, 0);
             }
         } else {
-            return fail(-1, "unknown src_kind %d", src_kind);
+            return set_error(-1, "unknown src_kind %d", src_kind);
         }
         SAD_CHECK_LAUNCH("k_wgrad_emb");
     }
