@@ -306,3 +306,42 @@ def test_gradient_of_time_major_rows_of_a_wider_matrix(save):
         got.append((y, grads[0]))
     for a, b in zip(*got):
         assert torch.equal(a, b) and a.transpose(0, 1).is_contiguous() and b.is_contiguous()
+
+
+@pytest.mark.parametrize("save", ["input", "int8"])
+def test_training_past_32_bits(save):
+    """Tensors of more than 2^32 bytes, forward and backward: the last sentences equal the same sentences alone (both calls are
+    uncut, so bit for bit)."""
+    torch, Fn = _t()
+    B, T, D, n = 1100, 650, 2048, 64
+    z = torch.zeros(B, T, 2 * D, dtype=torch.bfloat16, device="cuda")          # 5.9 GB
+    z[-n:].normal_()
+    z.requires_grad_(True)
+    dy = torch.empty(B, T, D, dtype=torch.bfloat16, device="cuda").normal_()
+    lengths = torch.full((B,), T, dtype=torch.int32, device="cuda")
+    lengths[-3:] = torch.tensor([0, 17, 600])
+    y, last = Fn.gated_scan(z, lengths=lengths, gated_output=False, save=save)
+    dz, = torch.autograd.grad([y, last], z, [dy, torch.ones_like(last)])
+    part = z.detach()[-n:].clone().requires_grad_(True)
+    yp, lp = Fn.gated_scan(part, lengths=lengths[-n:], gated_output=False, save=save)
+    dp, = torch.autograd.grad([yp, lp], part, [dy[-n:], torch.ones_like(lp)])
+    assert torch.equal(y[-n:], yp) and torch.equal(last[-n:], lp) and torch.equal(dz[-n:], dp)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_weight_grad_past_32_bits(dtype):
+    """dy of more than 2^32 bytes, small whole numbers: every sum is exact, so the rows of both ends alone give the same bits."""
+    torch, Fn = _t()
+    dt = getattr(torch, dtype)
+    M, N, K, n = 1_500_001, 1531, 40, 1000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randint(-63, 64, (M, K), device="cuda", generator=g).to(dt)
+    dy = torch.zeros(M, N, dtype=dt, device="cuda")
+    ends = [slice(0, n), slice(M - n, M)]
+    for e in ends:
+        dy[e] = torch.randint(-8, 9, (n, N), device="cuda", generator=g).to(dt)
+    dw, db = Fn.weight_grad8(dy, Fn.checkpoint8(x), bias=True)
+    xe, de = torch.cat([x[e] for e in ends]), torch.cat([dy[e] for e in ends])
+    ew, eb = Fn.weight_grad8(de, Fn.checkpoint8(xe), bias=True)
+    assert torch.equal(dw, ew) and torch.equal(db, eb)
+    assert torch.equal(ew.double(), de.double().t() @ xe.double()) and torch.equal(eb.double(), de.double().sum(0))
