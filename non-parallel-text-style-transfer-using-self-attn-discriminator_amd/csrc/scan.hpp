@@ -16,9 +16,11 @@
 // Bound by memory.  One wave owns 128 channels (two neighbours per lane: 4-byte loads, 256 contiguous bytes per row and part)
 // of one sentence and walks over time in blocks of 16 steps; the loads of the next block (48 instructions, 12 KB per wave)
 // are in flight while a block is computed.  16-bit types move 8 bytes per element forward (11 with 8-bit codes written) and
-// 14 backward (11 with codes read).  Measured, bf16: [8, 4096, 2048] with 8-bit activations, forward 144 us = 5.2 TB/s of
-// 754 MB, backward 156 us = 4.9 TB/s of 762 MB (a copy of 2 GB: 4.9 TB/s), their sums 80 and 84 us (3.4 TB/s);
-// [1024, 32, 512] ragged, forward 28 us, backward 36 us; [64, 23, 512] ragged 6.5 and 10 us (latency of two blocks).
+// 14 backward (11 with codes read).  Measured, bf16: [8, 4096, 2048] with 8-bit activations, forward 145 us = 5.2 TB/s of
+// 754 MB, backward 159 us = 4.8 TB/s of 762 MB (a copy of 2 GB: 4.9 TB/s), their sums 83 and 86 us (3.3 TB/s);
+// [1024, 32, 512] ragged, forward 28 us, backward 37 us; [64, 23, 512] ragged 6.6 and 10 us (latency of two blocks).
+// Channel counts whose rows do not start on lines cost more, as a wave's 256 bytes then lie in three lines instead of two: a
+// training call at [64, 500, 960] takes 171 us, at [64, 500, 1000] 207.
 //
 // A training call keeps the state that enters each block (fp32, 1/4 byte per element and step): the backward pass walks
 // the blocks from the last to the first, recomputes the 16 states of a block from its kept one in registers and needs
@@ -106,7 +108,8 @@ template <> struct Pair<SAD_SRC_F32> {
 // sigmoid(-f); exp2's overflow to infinity gives the limit 0
 __device__ __forceinline__ float sc_share(float f) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(SC_LOG2E * f)); }
 // u = 2^arg with arg kept where 1 + u and u / (1 + u) are finite; a NaN stays one (minimum, not min).  With arg = log2 e f:
-// 1 / (1 + u) = sigmoid(-f) and u / (1 + u) = sigmoid(f), each at full relative precision.
+// 1 / (1 + u) = sigmoid(-f) and u / (1 + u) = sigmoid(f), neither a difference from one: both keep a relative error of at most
+// (1.25 |f| + 8) 2^-24, most of it the rounding of the argument.
 __device__ __forceinline__ float sc_odds(float arg) { return __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(arg, 126.0f)); }
 
 // The part of a state (or of a carried gradient) that an update takes away from it, h - s h: an infinite one loses a finite

@@ -43,12 +43,11 @@ hipError_t allow_dynamic_lds(const void* kernel, int bytes) {
 
 // ---- scan ---------------------------------------------------------------------------------------------------------
 // Time chunks of a sentence: one where the waves of all sentences and channel groups fill the card by themselves (bf16, uncut
-// against cut: 800 waves of 300 steps, training 160 against 199 us, with 8-bit activations 216 against 234; 512 waves of 500
-// steps 224 against 212 and 323 against 237), or where a sentence is so short that the second launch costs more than the cut
+// against cut: 800 waves of 300 steps, training 160 against 200 us, with 8-bit activations 216 against 238; 512 waves of 500
+// steps 224 against 207 and 329 against 236), or where a sentence is so short that the second launch costs more than the cut
 // saves.  Otherwise as many as give 2048 waves at
-// most: what the backward kernel holds resident (two waves on each of 1024 SIMDs).  [8, 4096, 2048] with 8-bit
-// activations, us of all four kernels: 557 with 8 chunks, 463 with 16, 476 with 32, 566 with 18 (2304 waves: a second
-// round of 256).
+// most: what the backward kernel holds resident (two waves on each of 1024 SIMDs).  A training call at [8, 4096, 2048] with
+// 8-bit activations, us: 525 with 8 chunks, 433 with 16, 453 with 32, 557 with 18 (2304 waves: a second round of 256).
 int scan_chunks(int B, int T, int D) {
     const long long waves = (long long)B * ceil_div(D, SC_CH);
     const int nblk = ceil_div(T, SC_STEPS);

@@ -3,7 +3,7 @@
 // functional.py checks the arguments and calls these; they allocate, fill the argument structs and launch through libsad's
 // C-ABI.  They are here and not in Python because the calls are short: a backward pass runs on autograd's device thread, where
 // a Python node first has to take the interpreter lock from the thread that waits for it (a training call at [64, 23, 512]
-// took 115 us with Python nodes and takes 38).
+// took 115 us with Python nodes; it takes 37 us in some processes and 60 in others, as fast as that thread wakes).
 //
 // The library's functions are handed in as addresses (sad_amd::bind), so this file does not link libsad and follows whichever
 // build of it the package loaded.

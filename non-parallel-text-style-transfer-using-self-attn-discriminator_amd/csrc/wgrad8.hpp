@@ -17,11 +17,12 @@
 // fragment reads for the slices behind it, of the decoding and of the loads.  The compiler may not move instructions from
 // slice to slice (sched_barrier): left alone it reads all fragments first and decodes last.
 //
-// Measured, bf16: [16384 rows, 6144, 2048] 470-510 us (412 GFLOP: 810-880 TFLOP/s; a large library product reaches 1337, the
+// Measured, bf16: [16384 rows, 6144, 2048] 460-510 us (412 GFLOP: 810-900 TFLOP/s; a large library product reaches 1337, the
 // library's own dY^T X of this shape 943), matrix units busy 42 % of the cycles at a clock of 1.85-2.0 GHz under this load,
 // LDS 30 %, vector instructions 36 %, no bank conflicts; four waves of 96 x 128 outputs instead of eight of 96 x 64 read less
 // LDS but the compiler copies accumulators between register files (650 us).  [32768, 1536, 300]: 53 us and 8 us to
-// join 21 splits (the library: 188 us).
+// join 21 splits (the library: 188 us).  Rows of dY that no single stride reaches (a time-major dY under a batch-major
+// checkpoint) are read chunk by chunk behind the matrix loop: [64 x 500, 1536, 300] 61 us instead of 57.
 #pragma once
 #include "ckpt8.hpp"
 #include "gemm_core.hpp"
