@@ -171,8 +171,8 @@ def _lengths_to_device(src_len, B, device):
         if B > 0 and int(ln.min()) <= 0:
             raise RuntimeError("Length of all samples has to be greater than 0, but found an element in "
                                "'lengths' that is <= 0")
-        # as _own_int32; unpinned lengths through numpy, which costs less host time
-        own = _own_int32(src_len) if src_len.is_pinned() else torch.from_numpy(ln.astype(np.int32))
+        # as _own_int32; lengths of another type through numpy, which costs less host time and copies them anyway
+        own = _own_int32(src_len) if src_len.dtype == torch.int32 else torch.from_numpy(ln.astype(np.int32))
         return own.to(device=device, non_blocking=True)
     return src_len.to(device=device, dtype=torch.int32, non_blocking=True).contiguous()
 
