@@ -258,12 +258,27 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& z, const OptTensor& h0, cons
     return {y, h_last};
 }
 
+// do the address ranges of two non-empty matrices meet
+bool overlap(const Tensor& a, const Tensor& b) {
+    const auto end = [](const Tensor& t) {
+        return (const char*)t.data_ptr() + ((t.size(0) - 1) * t.stride(0) + (t.size(1) - 1) * t.stride(1) + 1) * (int64_t)t.element_size();
+    };
+    return (const char*)a.data_ptr() < end(b) && (const char*)b.data_ptr() < end(a);
+}
+
 // y; the new states go to h_out (h itself updates in place)
 Tensor gated_scan_step(const Tensor& z, const Tensor& h, const OptTensor& alive, bool gated, const Tensor& h_out) {
     no_tangent("gated_scan_step", z, h, h_out);
     const int64_t D = channels_of(z, "gated_scan_step", 2, gated);
     need_matrix(h, "gated_scan_step", "h", at::kFloat, z.size(0), D, z.device());
     need_matrix(h_out, "gated_scan_step", "h_out", at::kFloat, z.size(0), D, z.device());
+    // lanes read h and z while others write h_out
+    TORCH_CHECK(h_out.size(0) < 2 || h_out.stride(0) >= D, "gated_scan_step: rows of h_out overlap");
+    if (h.size(0) > 0) {
+        const bool same = h_out.data_ptr() == h.data_ptr() && h_out.strides() == h.strides();
+        TORCH_CHECK(same || !overlap(h_out, h), "gated_scan_step: h_out must be h itself or must not overlap it");
+        TORCH_CHECK(!overlap(h_out, z), "gated_scan_step: h_out must not overlap z");
+    }
     if (alive.has_value()) {
         need_vector(*alive, "gated_scan_step", "alive", z.size(0), z.device());
         TORCH_CHECK(alive->scalar_type() == at::kBool || alive->scalar_type() == at::kByte, "gated_scan_step: alive must be bool");

@@ -742,9 +742,10 @@ def gated_scan(z, h0=None, lengths=None, reverse=False, gated_output=True, save=
     makes it NaN.  ``lengths`` [B] (host or device, 0..T, any order): y is 0 at t >= length, the state
     stays, and such rows of z may hold anything.  ``reverse`` runs from the last token to the first.
 
-    Differentiable in z and h0, once and in reverse mode (dual tensors are refused).  ``save="input"`` keeps z for the backward pass; ``save="int8"`` keeps its 8-bit codes
-    instead (``checkpoint8``'s format, x, f and o separately) and gives the gradient at the restored values; both keep the
-    state entering every 16 tokens in float32, and a step between them is recomputed from there."""
+    Differentiable in z and h0, once and in reverse mode (dual tensors are refused).  ``save="input"`` keeps z for the
+    backward pass; ``save="int8"`` keeps its 8-bit codes instead (``checkpoint8``'s format, x, f and o separately) and gives
+    the gradient at the restored values; both keep the state entering every 16 tokens in float32, and a step between them is
+    recomputed from there."""
     _kind(z, "z")
     if z.dim() != 3:
         raise RuntimeError("z must be [B,T,3D] or [B,T,2D], got %s" % (tuple(z.shape),))

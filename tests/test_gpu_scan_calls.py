@@ -345,3 +345,20 @@ def test_weight_grad_past_32_bits(dtype):
     ew, eb = Fn.weight_grad8(de, Fn.checkpoint8(xe), bias=True)
     assert torch.equal(dw, ew) and torch.equal(db, eb)
     assert torch.equal(ew.double(), de.double().t() @ xe.double()) and torch.equal(eb.double(), de.double().sum(0))
+
+
+def test_step_operator_refuses_overlapping_states():
+    """The operator itself, past functional's checks: a shifted state would be read by some lanes after others wrote it."""
+    torch, Fn = _t()
+    from sad_amd import lib
+    step = lambda z, h, h_out: lib.load_ops().gated_scan_step(z, h, None, True, h_out)
+    z, buf = torch.zeros(2, 12, device="cuda"), torch.zeros(3, 4, device="cuda")
+    flat = torch.zeros(24, device="cuda")
+    for args, message in (((z, buf[:2], buf[1:]), "must not overlap it"), ((z, buf[1:], buf[:2]), "must not overlap it"),
+                          ((z, buf[:2], torch.zeros(1, 4, device="cuda").expand(2, 4)), "rows of h_out overlap"),
+                          ((flat.view(2, 12), buf[:2], flat[16:].view(2, 4)), "must not overlap z")):
+        with pytest.raises(RuntimeError, match=message):
+            step(*args)
+    step(z, buf[:2], buf[:2])
+    step(z, torch.zeros(1, 4, device="cuda").expand(2, 4), buf[:2])
+    step(z[:1], buf[:1], buf[1:2])
